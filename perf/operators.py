@@ -109,13 +109,13 @@ def half_of_byte(device):
 
 def quantize(x):
     """Codes (packed, two a byte) and scale bytes of float32 numbers ``[..., dim]``."""
-    table = half_of_byte(x.device)[:LARGEST + 1].contiguous()
+    table = half_of_byte(x.device)[:LARGEST + 1] / SCALE_STEPS
     groups = x.unflatten(-1, (-1, GROUP))
     most = groups.abs().amax(-1)
     finite = torch.isfinite(most)
-    wanted = torch.where(finite, most / 7.0 * SCALE_STEPS, torch.zeros_like(most))
-    scale = torch.searchsorted(table, wanted).clamp(max=LARGEST)             # the smallest that is not below
-    inverse = torch.where(scale > 0, 1.0 / (table[scale] / SCALE_STEPS), torch.zeros_like(most))
+    # the smallest scale of which seven steps reach the largest number (seven times a scale is exact)
+    scale = torch.searchsorted(7.0 * table, torch.where(finite, most, torch.zeros_like(most))).clamp(max=LARGEST)
+    inverse = torch.where(scale > 0, 1.0 / table[scale], torch.zeros_like(most))
     codes = (groups * inverse[..., None]).round().clamp(-7.0, 7.0)
     codes = torch.where(finite[..., None], codes, torch.zeros_like(codes)).to(torch.int16).flatten(-2) + 8
     packed = (codes[..., 0::2] | (codes[..., 1::2] << 4)).to(torch.uint8)
@@ -274,7 +274,7 @@ def exact_rounded(x):
     """Float64 numbers ``[..., dim]`` brought to the nearest number that the cache holds."""
     scales = exact_scales(x.device)[:LARGEST + 1].contiguous()
     groups = x.reshape(x.shape[:-1] + (-1, 16))
-    step = scales[torch.searchsorted(scales, groups.abs().amax(-1) / 7.0).clamp(max=LARGEST)][..., None]
+    step = scales[torch.searchsorted(7.0 * scales, groups.abs().amax(-1)).clamp(max=LARGEST)][..., None]
     return (torch.clamp(torch.round(groups / step.clamp(min=1e-30)), -7, 7) * step).reshape(x.shape)
 
 
