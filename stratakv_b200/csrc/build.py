@@ -26,11 +26,12 @@ from pathlib import Path
 from typing import Optional
 
 CSRC = Path(__file__).resolve().parent
-HEAD_SOURCES = ("attention.cu", "attention_decode.cu", "attention_decode_fused.cu", "attention_prefill.cu", "attention_prefill_tc.cu")
+HEAD_SOURCES = ("attention.cu", "attention_decode.cu", "attention_decode_fused.cu", "attention_prefill.cu", "attention_prefill_tc.cu",
+                "attention_kv4.cu")
 COMMON_SOURCES = ("elementwise.cu", "linear.cu", "gemm_tcgen05.cu", "attention_general.cu", "sampling.cu", "stream_ops.cu",
                   "headwise_linear.cu", "recurrent.cu", "stream_mix.cu", "retention.cu", "latent_finish.cu", "routed_mlp.cu",
-                  "short_conv.cu", "time_mix.cu", "normed_rotary.cu", "linear_state.cu", "channel_state.cu")
-HEADERS = ("common.cuh", "head_size.cuh")
+                  "short_conv.cu", "time_mix.cu", "normed_rotary.cu", "linear_state.cu", "channel_state.cu", "kv4.cu")
+HEADERS = ("common.cuh", "head_size.cuh", "kv4.cuh")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 COMMON_FLAGS = ("-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden")
 DTYPE_CODES = {"float32": 0, "bfloat16": 1}

@@ -1,0 +1,367 @@
+"""The kernels of a cache held in 4 bits against plain computations: what is stored equals the plain form's bytes, what is read back is
+exact, and attention is compared with 64 bits."""
+import math
+
+import pytest
+import torch
+
+import plain_kv4
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = 2.0 ** -8                          # a rounding to bfloat16, relative
+
+
+def lib(head_dim):
+    from stratakv_b200.ops import kernels_for
+    return kernels_for(torch.bfloat16, head_dim, verbose=False)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def make_cache(kv, dim, block, lengths, fill=0xFF, spread=1.0, spare=3):
+    """Paged codes and scales whose live rows hold random numbers; everything else is ``fill`` (0xFF: scales of NaN)."""
+    width = max(1, -(-max(lengths) // block))
+    total = len(lengths) * width + spare
+    table = torch.randperm(total, device="cuda")[:len(lengths) * width].int().view(len(lengths), width).contiguous()
+    cache = [torch.full((total, kv, block, w), fill, dtype=torch.uint8, device="cuda") for w in (dim // 2, dim // 2, dim // 16, dim // 16)]
+    for s, length in enumerate(lengths):
+        for of in (0, 1):
+            codes, scale = plain_kv4.store(torch.randn(kv, length, dim, device="cuda") * spread)
+            for b in range(-(-length // block)):
+                rows = min(block, length - b * block)
+                cache[of][table[s, b], :, :rows] = codes[:, b * block:b * block + rows]
+                cache[2 + of][table[s, b], :, :rows] = scale[:, b * block:b * block + rows]
+    return cache, table
+
+
+def cached(cache, table, s, length, block, of):
+    """Float64 ``[kv_heads, length, dim]``: keys (of 0) or values (of 1) of sequence s."""
+    blocks = table[s, :-(-length // block)].long()
+    return plain_kv4.read(cache[of][blocks], cache[2 + of][blocks]).transpose(0, 1).flatten(1, 2)[:, :length]
+
+
+# ---- appending ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,kv,dim,block,new,rotated", [
+    (4, 2, 16, 16, [1], True), (3, 3, 80, 64, [5, 1, 70], True), (8, 2, 128, 32, [1] * 9, True), (7, 1, 64, 16, [33, 16, 15], False),
+    (32, 8, 128, 64, [130], True), (5, 1, 208, 16, [3, 17], True), (2, 2, 256, 32, [31], False)])
+def test_append_stores_the_plain_forms_bytes(heads, kv, dim, block, new, rotated):
+    from stratakv_b200.parts.position import rope_table
+    k = lib(dim)
+    before = [7 * i + 3 for i in range(len(new))]
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, dim, block, lengths, fill=0xA5)
+    kept = [c.clone() for c in cache]
+    n = sum(new)
+    # loud and quiet groups, and some of zeros
+    qkv = torch.randn(n, (heads + 2 * kv) * dim, device="cuda") * torch.exp2(torch.randint(-12, 9, (n, (heads + 2 * kv) * dim // 16), device="cuda").float()).repeat_interleave(16, 1)
+    qkv[:, -16:] = 0.0
+    positions = torch.cat([torch.arange(b, b + c) for b, c in zip(before, new)]).int().cuda()
+    seqs = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new)).int().cuda()
+    cos_sin = torch.from_numpy(rope_table(dim, 10000.0, max(lengths))).cuda() if rotated else None
+    q_out = torch.full((n, heads * dim), float("nan"), device="cuda").bfloat16()
+    k.append_kv4(qkv, cos_sin, positions, seqs, table, q_out, *cache, heads, kv, dim, block)
+    rows = qkv.view(n, heads + 2 * kv, dim)
+    turned = plain_kv4.rotate(rows[:, :heads + kv], cos_sin, positions)
+    assert torch.equal(q_out, turned[:, :heads].flatten(1).bfloat16())
+    blocks, at = table[seqs.long(), positions.long() // block].long(), positions.long() % block
+    for of, x in ((0, turned[:, heads:]), (1, rows[:, heads + kv:])):
+        codes, scale = plain_kv4.store(x)
+        kept[of][blocks, :, at], kept[2 + of][blocks, :, at] = codes, scale
+        # and what they stand for is the nearest of the numbers that their group's smallest sufficient scale has
+        near = plain_kv4.read(codes, scale)
+        step = plain_kv4.scale_table("cuda")[scale.long()].repeat_interleave(16, dim=-1)
+        assert bool(((near - x.double()).abs() <= step * (0.5 + 2.0 ** -20)).all())
+        assert bool((step * 7 * (1 + 2.0 ** -22) >= x.double().abs()).all())
+    for mine, plain in zip(cache, kept):
+        assert torch.equal(mine, plain)            # (nothing else was touched)
+
+
+def test_append_at_the_borders_of_its_scales():
+    """Groups whose largest number is 7 times a scale, and its neighbours; the largest and smallest numbers; what is not finite."""
+    dim, block = 64, 16
+    k = lib(dim)
+    table64 = plain_kv4.scale_table()[1:plain_kv4.LARGEST + 1]
+    exact = (table64 * 7).float()
+    most = torch.cat([exact, torch.nextafter(exact, exact * 2), torch.nextafter(exact, exact * 0), torch.tensor([0.0, 1e-30, 1e-40, 6272.0, 6273.0, 1e9, 3.4e38])])
+    n = -(-most.numel() // 4)
+    values = torch.zeros(n, 4, 16)
+    values.view(-1, 16)[:most.numel(), 3] = -most
+    values.view(-1, 16)[:most.numel(), 7] = most * 0.5           # (half a step off two codes: ties go to the even one)
+    qkv = torch.cat([torch.zeros(n, dim), torch.zeros(n, dim), values.flatten(1)], dim=1).cuda()
+    special = qkv[:6].clone()
+    special[:, dim:] = torch.randn(6, 2 * dim, device="cuda")
+    for i, bad in enumerate([math.inf, -math.inf, math.nan, math.inf, math.nan, 1.0]):
+        special[i, dim + 16 * (i % 4) + i] = bad
+        special[i, 2 * dim + 5] = bad
+    qkv = torch.cat([qkv, special]).contiguous()
+    n = qkv.shape[0]
+    cache, table = make_cache(1, dim, block, [n])
+    q_out = torch.empty(n, dim, dtype=torch.bfloat16, device="cuda")
+    k.append_kv4(qkv, None, torch.arange(n, device="cuda", dtype=torch.int32), torch.zeros(n, device="cuda", dtype=torch.int32), table, q_out,
+                 *cache, 1, 1, dim, block)
+    for of in (0, 1):
+        codes, scale = plain_kv4.store(qkv[:, dim * (1 + of):dim * (2 + of)])
+        blocks, at = table[0, torch.arange(n) // block].long(), torch.arange(n) % block
+        assert torch.equal(cache[2 + of][blocks, 0, at], scale) and torch.equal(cache[of][blocks, 0, at], codes)
+    out = [torch.empty(table.shape[1], 1, block, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    k.unpack_kv4(*cache, table, ints([n]), *out, torch.empty_like(table), 1, dim, block)
+    read = out[1].view(-1, dim)[:n].float().cpu()
+    assert read[:n - 6].abs().max() == 6272.0 and bool(torch.isfinite(read[:n - 6]).all())
+    assert bool(torch.isnan(read[n - 6:n - 1, :16]).all()) and bool(torch.isfinite(read[n - 1]).all()) and bool(torch.isfinite(read[n - 6:, 16:]).all())
+
+
+def test_append_of_queries_alone_leaves_the_cache():
+    k = lib(64)
+    cache, table = make_cache(1, 64, 16, [20])
+    kept = [c.clone() for c in cache]
+    qkv = torch.randn(4, 4 * 64, device="cuda")
+    q_out = torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")
+    k.append_kv4(qkv, None, torch.arange(4, device="cuda", dtype=torch.int32), ints([0] * 4), table, q_out, *cache, 2, 1, 64, 16, write_kv=False)
+    assert torch.equal(q_out, qkv[:, :128].bfloat16()) and all(torch.equal(a, b) for a, b in zip(cache, kept))
+
+
+# ---- reading back ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kv,dim,block,lengths,keep,width", [
+    (2, 16, 16, [1], 0, 1), (3, 80, 64, [64, 65, 1, 200], 0, 4), (1, 128, 16, [100, 17, 16, 33], 17, 3), (2, 64, 32, [130, 31], 1, 1),
+    (2, 64, 32, [130, 31], 64, 3), (1, 256, 16, [40], 0, 5)])
+def test_unpack_gives_what_the_codes_stand_for(kv, dim, block, lengths, keep, width):
+    k = lib(dim)
+    cache, table = make_cache(kv, dim, block, lengths)
+    n = len(lengths)
+    out = [torch.full((n * width, kv, block, dim), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    out_table = torch.full_like(table, -7)
+    k.unpack_kv4(*cache, table, ints(lengths), *out, out_table, kv, dim, block, keep)
+    for s, length in enumerate(lengths):
+        first = max(0, length - keep) // block if keep else 0
+        for of in (0, 1):
+            plain = cached(cache, table, s, length, block, of)
+            wanted = torch.zeros(kv, width * block, dim, dtype=torch.float64, device="cuda")
+            some = plain[:, first * block:first * block + width * block]
+            wanted[:, :some.shape[1]] = some
+            got = out[of].view(n, width, kv, block, dim)[s].transpose(0, 1).flatten(1, 2)
+            assert torch.equal(got.double(), wanted)
+        for b in range(table.shape[1]):
+            assert int(out_table[s, b]) == (s * width + b - first if first <= b < first + width else 0)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+
+def check_attention(heads, kv, dim, block, before, new, window=0, spread=1.0, extra_rows=0, table_room=0):
+    k = lib(dim)
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, dim, block, lengths, spread=spread)
+    if table_room:
+        table = torch.cat([table, torch.zeros(table.shape[0], table_room, dtype=torch.int32, device="cuda")], dim=1).contiguous()
+    tokens = sum(new)
+    q = torch.randn(tokens + extra_rows, heads * dim, device="cuda").bfloat16()
+    out = torch.full((tokens + extra_rows, heads * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    cu = [0]
+    for c in new:
+        cu.append(cu[-1] + c)
+    scale = 1.0 / math.sqrt(dim)
+    wanted = k.attention_kv4_scratch(len(new), q.shape[0], max(new), table.shape[1], heads, kv, dim, block, window)
+    scratch = torch.full((wanted,), 0xFF, dtype=torch.uint8, device="cuda")
+    k.attention_kv4(q, *cache, table, ints(cu), ints(lengths), out, max(new), heads, kv, dim, block, scale, window, scratch)
+    unpacked = k._kv4_unpacked_width(len(new), max(new), table.shape[1], heads, kv, dim, block, window) > 0
+    for s in range(len(new)):
+        ref, sums, whole = plain_kv4.attention(q[cu[s]:cu[s + 1]].double().view(new[s], heads, dim), cached(cache, table, s, lengths[s], block, 0),
+                                        cached(cache, table, s, lengths[s], block, 1), before[s], scale, window)
+        got = out[cu[s]:cu[s + 1]].double().view(new[s], heads, dim)
+        # The result is rounded once; a probability keeps 11 bits (8 behind unpack_kv4), its exponential and the
+        # sums of products together another 2^-11 of what is added up.  A half below 2^-14 is a multiple of 2^-24: a probability, which is
+        # held 2^7 times as large as it is next to the row's largest (the maximum in use is never above the largest), is off by at
+        # most half of that over 2^7 there, 2^-32, and so is its key's share of the result next to a denominator of at least 1.
+        # (Weights of nearly nothing show where the keys that have the weight hold zeros.)
+        allowed = HALF_STEP * ref.abs() + ((2.0 ** -8 if unpacked else 2.0 ** -11) + 2.0 ** -11) * sums + 2.0 ** -32 * whole
+        assert bool(((got - ref).abs() <= allowed).all()), (s, float(((got - ref).abs() / allowed).max()))
+    assert bool((out[tokens:] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,kv,dim,block,lengths,window", [
+    (4, 2, 16, 16, [1], 0), (3, 3, 80, 64, [5, 64, 65, 130], 0), (8, 2, 128, 32, [1, 15, 16, 17, 300], 0), (32, 4, 64, 64, [2048, 3, 511], 0),
+    (7, 1, 64, 16, [100, 257], 40), (24, 1, 128, 16, [77, 1000], 0), (32, 32, 128, 16, [200, 1, 45], 0), (2, 1, 208, 16, [129, 64], 0),
+    (4, 1, 256, 64, [300], 17), (6, 2, 48, 32, [33, 500], 1), (32, 8, 128, 64, [9000], 1024), (2, 1, 192, 16, [70], 0)])
+def test_attention_of_one_token_a_sequence(heads, kv, dim, block, lengths, window):
+    check_attention(heads, kv, dim, block, [n - 1 for n in lengths], [1] * len(lengths), window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,block,before,new,window", [
+    (8, 2, 128, 32, [0, 40, 100], [1, 3, 5], 0), (4, 4, 64, 16, [0, 7, 300], [16, 2, 9], 0), (3, 1, 80, 64, [62, 0], [5, 20], 0),
+    (8, 1, 64, 64, [1000], [8], 33), (32, 8, 128, 16, [4000, 511], [5, 1], 0), (2, 1, 16, 48, [10], [70], 20), (2, 2, 208, 16, [3, 0], [9, 40], 0),
+    (4, 2, 128, 48, [90], [50], 0)])
+def test_attention_of_a_few_tokens_a_sequence(heads, kv, dim, block, before, new, window):
+    check_attention(heads, kv, dim, block, before, new, window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,block,before,new,window", [
+    (4, 2, 64, 64, [0], [300], 0), (4, 1, 128, 16, [77, 0, 900], [130, 1, 40], 0), (8, 8, 64, 32, [1000, 5], [65, 200], 100),
+    (2, 1, 128, 128, [3], [513], 64), (8, 2, 64, 64, [0] * 5, [100, 1, 64, 65, 33], 0)])
+def test_attention_of_prompts(heads, kv, dim, block, before, new, window):
+    check_attention(heads, kv, dim, block, before, new, window)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [4, 2], [100, 30]])
+def test_attention_leaves_rows_behind_the_last_sequence(new):
+    check_attention(4, 2, 64, 32, [3000, 600], new, extra_rows=5, table_room=3)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spread", [1e-4, 40.0])
+def test_attention_over_quiet_and_loud_caches(dim, spread):
+    """Scores of nearly nothing, and scores that leave one key (whose neighbours' probabilities vanish)."""
+    check_attention(4, 1, dim, 16, [700, 40], [1, 1], spread=spread)
+
+
+def run_step(k, q, cache, table, cu, ctx, heads, kv, dim, block, most, window=0):
+    out = torch.empty_like(q)
+    scratch = torch.full((k.attention_kv4_scratch(len(ctx), q.shape[0], most, table.shape[1], heads, kv, dim, block, window),), 0xFF, dtype=torch.uint8, device="cuda")
+    k.attention_kv4(q, *cache, table, ints(cu), ints(ctx), out, most, heads, kv, dim, block, 1.0 / math.sqrt(dim), window, scratch)
+    return out
+
+
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("at", [0, 500, 998])
+def test_what_is_not_finite_reaches_the_rows_that_see_it_alone(dim, at):
+    """A value's NaN in one group of one position: only that group's numbers, only of queries at or behind that position; a key's NaN
+    reaches all of such a query's numbers.  With a window, queries that have left it behind stay clean."""
+    k = lib(dim)
+    heads, kv, block, before, new = 4, 2, 16, 995, 5
+    cache, table = make_cache(kv, dim, block, [before + new])
+    q = torch.randn(new, heads * dim, device="cuda").bfloat16()
+    clean = run_step(k, q, cache, table, [0, new], [before + new], heads, kv, dim, block, new, window=997)
+    entry = table[0, at // block].long()
+    spoiled = [c.clone() for c in cache]
+    spoiled[3][entry, 1, at % block, 2] = plain_kv4.NOT_FINITE
+    got = run_step(k, q, spoiled, table, [0, new], [before + new], heads, kv, dim, block, new, window=997).view(new, heads, dim)
+    sees = torch.tensor([at <= before + i and at > before + i - 997 for i in range(new)])
+    wanted = torch.zeros(new, heads, dim, dtype=torch.bool)
+    wanted[:, 2:, 32:48] = sees[:, None, None]
+    assert torch.equal(torch.isnan(got).cpu(), wanted)
+    assert torch.equal(got[~wanted.cuda()], clean.view(new, heads, dim)[~wanted.cuda()])
+    spoiled = [c.clone() for c in cache]
+    spoiled[2][entry, 0, at % block, 1] = plain_kv4.NOT_FINITE
+    got = run_step(k, q, spoiled, table, [0, new], [before + new], heads, kv, dim, block, new, window=997).view(new, heads, dim)
+    wanted = torch.zeros(new, heads, dim, dtype=torch.bool)
+    wanted[:, :2] = sees[:, None, None]
+    assert torch.equal(torch.isnan(got).cpu(), wanted)
+    assert torch.equal(got[~wanted.cuda()], clean.view(new, heads, dim)[~wanted.cuda()])
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_query_that_is_not_finite_gives_nan_and_spoils_no_other(bad):
+    k = lib(64)
+    cache, table = make_cache(1, 64, 16, [600, 600])
+    q = torch.randn(2, 4 * 64, device="cuda").bfloat16()
+    clean = run_step(k, q, cache, table, [0, 1, 2], [600, 600], 4, 1, 64, 16, 1)
+    q[0, 64 + 3] = bad
+    got = run_step(k, q, cache, table, [0, 1, 2], [600, 600], 4, 1, 64, 16, 1)
+    assert bool(torch.isnan(got[0, 64:128]).all())
+    got[0, 64:128] = clean[0, 64:128]
+    assert torch.equal(got, clean)
+
+
+def test_queries_of_any_size():
+    """Powers of two on a query and off the scale change nothing but the products' exponents."""
+    k = lib(128)
+    cache, table = make_cache(1, 128, 64, [333])
+    q = torch.randn(1, 2 * 128, device="cuda").bfloat16()
+    plain = run_step(k, q, cache, table, [0, 1], [333], 2, 1, 128, 64, 1)
+    for power in (-90, -20, 30, 100):
+        out = torch.empty_like(q)
+        scratch = torch.empty(k.attention_kv4_scratch(1, 1, 1, table.shape[1], 2, 1, 128, 64), dtype=torch.uint8, device="cuda")
+        k.attention_kv4((q.float() * 2.0 ** power).bfloat16(), *cache, table, ints([0, 1]), ints([333]), out, 1, 2, 1, 128, 64,
+                        2.0 ** -power / math.sqrt(128), 0, scratch)
+        assert torch.equal(out, plain), power
+
+
+def test_a_long_context_beyond_32_bit_offsets():
+    """Blocks whose bytes lie beyond 2^31 from the cache's start."""
+    dim, kv, block = 128, 8, 64
+    k = lib(dim)
+    blocks = (2 ** 31 // (kv * block * dim // 2)) + 40
+    cache = [torch.zeros(blocks, kv, block, w, dtype=torch.uint8, device="cuda") for w in (64, 64, 8, 8)]
+    table = torch.arange(blocks - 8, blocks, device="cuda", dtype=torch.int32)[None].contiguous()
+    length = 8 * block - 5
+    for of in (0, 1):
+        codes, scale = plain_kv4.store(torch.randn(8, kv, block, dim, device="cuda"))
+        cache[of][blocks - 8:], cache[2 + of][blocks - 8:] = codes, scale
+    q = torch.randn(1, 8 * dim, device="cuda").bfloat16()
+    out = run_step(k, q, cache, table, [0, 1], [length], 8, kv, dim, block, 1)
+    ref, sums, _ = plain_kv4.attention(q.double().view(1, 8, dim), cached(cache, table, 0, length, block, 0), cached(cache, table, 0, length, block, 1),
+                                    length - 1, 1.0 / math.sqrt(dim))
+    assert bool(((out.double().view(1, 8, dim) - ref).abs() <= HALF_STEP * ref.abs() + 2.0 ** -10 * sums).all())
+
+
+def test_append_read_back_and_attend_together():
+    """A prompt, then single tokens, as they would be used: each step's result equals attention over what the plain form stores."""
+    from stratakv_b200.parts.position import rope_table
+    heads, kv, dim, block = 8, 2, 64, 16
+    k = lib(dim)
+    cache, table = make_cache(kv, dim, block, [160, 160])
+    cos_sin = torch.from_numpy(rope_table(dim, 10000.0, 160)).cuda()
+    stored = [[], []]
+    before = [0, 0]
+    for new in ([100, 37], [1, 1], [3, 2], [1, 1], [40, 1]):
+        n = sum(new)
+        qkv = torch.randn(n, (heads + 2 * kv) * dim, device="cuda")
+        positions = torch.cat([torch.arange(b, b + c) for b, c in zip(before, new)]).int().cuda()
+        seqs = torch.repeat_interleave(torch.arange(2), torch.tensor(new)).int().cuda()
+        q = torch.empty(n, heads * dim, dtype=torch.bfloat16, device="cuda")
+        k.append_kv4(qkv, cos_sin, positions, seqs, table, q, *cache, heads, kv, dim, block)
+        after = [b + c for b, c in zip(before, new)]
+        cu = [0, new[0], n]
+        out = run_step(k, q, cache, table, cu, after, heads, kv, dim, block, max(new))
+        rows = qkv.view(n, heads + 2 * kv, dim)
+        turned = plain_kv4.rotate(rows[:, :heads + kv], cos_sin, positions)
+        for s in range(2):
+            mine = slice(cu[s], cu[s + 1])
+            stored[s].append([plain_kv4.read(*plain_kv4.store(x[mine])) for x in (turned[:, heads:], rows[:, heads + kv:])])
+            keys, values = (torch.cat([piece[i] for piece in stored[s]]).transpose(0, 1) for i in (0, 1))
+            ref, sums, _ = plain_kv4.attention(turned[mine, :heads].bfloat16().double(), keys, values, before[s], 1.0 / math.sqrt(dim))
+            allowed = HALF_STEP * ref.abs() + (2.0 ** -8 + 2.0 ** -11) * sums
+            assert bool(((out[mine].double().view(new[s], heads, dim) - ref).abs() <= allowed).all())
+        before = after
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------------------
+
+def test_refusals():
+    from stratakv_b200.ops import KernelError
+    k = lib(64)
+    cache, table = make_cache(2, 64, 16, [40])
+    q = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty_like(q)
+
+    def attend(**change):
+        a = dict(q=q, k_codes=cache[0], v_codes=cache[1], k_scale=cache[2], v_scale=cache[3], block_table=table, cu_q=ints([0, 1]), ctx_after=ints([40]),
+                 out=out, max_q_len=1, num_heads=4, num_kv_heads=2, head_dim=64, block_size=16, scale=0.125, window=0, scratch=None)
+        a.update(change)
+        k.attention_kv4(**a)
+
+    attend()
+    for match, change in (("heads must be a positive multiple", dict(num_heads=5, q=torch.zeros(1, 320, dtype=torch.bfloat16, device="cuda"), out=torch.zeros(1, 320, dtype=torch.bfloat16, device="cuda"))),
+                          ("k_codes must be", dict(k_codes=cache[2])), ("v_scale must be torch.uint8", dict(v_scale=cache[3].float())),
+                          ("one length, one offset pair", dict(cu_q=ints([0, 1, 1]))), ("q and out must be", dict(out=out[:, :128].contiguous())),
+                          ("a window must not be negative", dict(window=-1)), ("must be torch.bfloat16", dict(q=q.float())),
+                          ("must be contiguous", dict(block_table=torch.cat([table, table], dim=1)[:, ::2])), ("CUDA tensor", dict(q=q.cpu()))):
+        with pytest.raises(KernelError, match=match):
+            attend(**change)
+    long_cache, long_table = make_cache(2, 64, 16, [4000])
+    with pytest.raises(KernelError, match="bytes of scratch are needed"):
+        attend(k_codes=long_cache[0], v_codes=long_cache[1], k_scale=long_cache[2], v_scale=long_cache[3], block_table=long_table, ctx_after=ints([4000]),
+               scratch=torch.empty(8, dtype=torch.uint8, device="cuda"))
+    qkv = torch.zeros(1, 8 * 64, device="cuda")
+    with pytest.raises(KernelError, match="width does not match"):
+        k.append_kv4(qkv[:, :256].contiguous(), None, ints([0]), ints([0]), table, out, *cache, 4, 2, 64, 16)
+    with pytest.raises(KernelError, match="one query row"):
+        k.append_kv4(qkv, None, ints([0, 1]), ints([0]), table, out, *cache, 4, 2, 64, 16)
+    blocks = torch.empty(3, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(KernelError, match="positions to keep"):
+        k.unpack_kv4(*cache, table, ints([40]), blocks, blocks.clone(), torch.empty_like(table), 2, 64, 16, -1)
+    with pytest.raises(KernelError, match="results must be"):
+        k.unpack_kv4(*cache, table, ints([40]), blocks, blocks[:2].contiguous(), torch.empty_like(table), 2, 64, 16)
