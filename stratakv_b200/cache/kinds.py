@@ -14,7 +14,9 @@ token-major blocks (``include/stratakv/layers/attention.h:88-91``).
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Callable, Dict, Tuple
+from typing import Callable, Dict, Optional, Tuple
+
+import torch
 
 Shapes = Dict[str, Tuple[int, ...]]
 
@@ -23,11 +25,13 @@ Shapes = Dict[str, Tuple[int, ...]]
 class CacheKind:
     """``block_tensors(request, block_size)`` returns, by tensor name, the shape of ONE block of ONE cache
     entry; the cache puts ``[entries, blocks + 1]`` in front.  ``paged`` false: nothing is kept per
-    position (fixed-size state only).  ``windowed``: blocks behind ``request.window`` are given back."""
+    position (fixed-size state only).  ``windowed``: blocks behind ``request.window`` are given back.
+    ``dtype``: what the tensors hold where it is not the cache's own dtype."""
     name: str
     paged: bool
     windowed: bool
     block_tensors: Callable[..., Shapes]
+    dtype: Optional[torch.dtype] = None
 
 
 _KINDS: Dict[str, CacheKind] = {}
@@ -54,4 +58,15 @@ def _keys_and_values(request, block_size: int) -> Shapes:
 
 register_cache_kind(CacheKind("kv", paged=True, windowed=False, block_tensors=_keys_and_values))
 register_cache_kind(CacheKind("kv_window", paged=True, windowed=True, block_tensors=_keys_and_values))
+
+
+def _keys_and_values_in_4_bits(request, block_size: int) -> Shapes:
+    """Two codes a byte, and a scale byte for each 16 numbers (``csrc/kv4.cuh``)."""
+    tile = lambda width: (request.num_kv_heads, block_size, width)
+    return {"k": tile(request.head_dim // 2), "v": tile(request.head_dim // 2),
+            "k_scale": tile(request.head_dim // 16), "v_scale": tile(request.head_dim // 16)}
+
+
+register_cache_kind(CacheKind("kv4", paged=True, windowed=False, block_tensors=_keys_and_values_in_4_bits, dtype=torch.uint8))
+register_cache_kind(CacheKind("kv4_window", paged=True, windowed=True, block_tensors=_keys_and_values_in_4_bits, dtype=torch.uint8))
 register_cache_kind(CacheKind("none", paged=False, windowed=False, block_tensors=lambda request, block_size: {}))

@@ -93,8 +93,8 @@ class KVCache:
         for group in self.groups:
             # one block more than the allocator hands out: padding rows of a step write there
             for name, shape in group.kind.block_tensors(group.request, block_size).items():
-                group.storage[name] = torch.zeros((len(group.entries), num_blocks + 1) + tuple(shape), dtype=dtype,
-                                                  device=self.device)
+                group.storage[name] = torch.zeros((len(group.entries), num_blocks + 1) + tuple(shape),
+                                                  dtype=group.kind.dtype or dtype, device=self.device)
         # Fixed-size per-sequence state, one row per slot for each entry that asks for some.
         self.state_bytes = [r.state_bytes for r in requests]
         # (one row more than there are slots: padding rows of a graph step name it, so that a part which

@@ -38,7 +38,10 @@ class EngineConfig:
     ``max_position_embeddings``, a positive value replaces it (the rotary
     encoding is defined at any position; what lies beyond the model's own limit
     is the caller's decision).  The reference's only such limit is its cache
-    capacity (``src/generation/generator.cpp:628-632``)."""
+    capacity (``src/generation/generator.cpp:628-632``).  ``cache_dtype``: what keys
+    and values are kept in, the compute dtype ("" or its name) or "int4": 4 bits and
+    a scale byte for each 16 numbers, 0.28 of bfloat16's bytes (bfloat16 models all
+    of whose cached layers are plain attention)."""
     max_tokens: int
     dtype: torch.dtype = torch.bfloat16
     block_size: int = 64
@@ -46,6 +49,7 @@ class EngineConfig:
     device: str = "cuda:0"
     use_cuda_graphs: bool = True
     max_context: int = 0
+    cache_dtype: str = ""
 
     def __post_init__(self):
         if self.max_tokens <= 0:
@@ -57,6 +61,10 @@ class EngineConfig:
         if self.max_context < 0:
             raise ConfigError("max_context must be non-negative")
         object.__setattr__(self, "dtype", parse_dtype(self.dtype))
+        if self.cache_dtype not in ("", "int4") and parse_dtype(self.cache_dtype) != self.dtype:
+            raise ConfigError(f"cache_dtype must be the compute dtype or int4, got {self.cache_dtype!r}")
+        if self.cache_dtype == "int4" and self.dtype != torch.bfloat16:
+            raise ConfigError("a cache held in 4 bits is read by the bfloat16 kernels alone")
 
     @property
     def num_blocks(self) -> int:

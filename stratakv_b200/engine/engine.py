@@ -22,8 +22,10 @@ from .. import models as _models  # noqa: F401  (registers the architectures)
 from .. import ops as _ops
 from ..cache import CacheFull, KVCache
 from ..config import EngineConfig, load_config
+from ..config.llama import ConfigError
 from ..config.registry import resolve_architecture
 from ..parts.base import Runtime, StepBatch
+from ..parts.registry import part_class
 from ..parts.spec import ModelSpec
 from ..parts.workspace import Workspace
 from ..weights.loader import load_checkpoint
@@ -67,7 +69,7 @@ def _token_array(tokens) -> np.ndarray:
 class Engine:
     def __init__(self, spec: ModelSpec, tensors: Mapping[str, torch.Tensor], config: EngineConfig,
                  kernel_loader=None, verbose: bool = True):
-        self.spec = spec
+        spec = self.spec = self._kept_in(spec, config)
         self.config = config
         # most positions a sequence may reach: the engine's setting, else the model's own limit, else none
         self.max_context = config.max_context or spec.max_positions or 0
@@ -107,6 +109,23 @@ class Engine:
             import dataclasses
             return dataclasses.replace(config, dtype=torch.float32)
         return config
+
+    @staticmethod
+    def _kept_in(spec: ModelSpec, config: EngineConfig) -> ModelSpec:
+        """The description with its keys and values kept as the configuration wants them."""
+        if config.cache_dtype != "int4":
+            return spec
+        import dataclasses
+        layers = []
+        for layer in spec.layers:
+            mixer = layer.mixer
+            if mixer is not None and part_class("mixer", mixer.kind).cache_request(mixer).kind != "none":
+                if mixer.kind != "attention" or mixer.extended or mixer.head_dim % 16:
+                    raise ConfigError(f"a cache held in 4 bits serves layers of plain attention (heads a multiple of 16 wide); "
+                                      f"this model has a '{mixer.kind}' layer that keeps something else")
+                layer = dataclasses.replace(layer, mixer=dataclasses.replace(mixer, cache_bits=4))
+            layers.append(layer)
+        return dataclasses.replace(spec, layers=type(spec.layers)(layers))
 
     @classmethod
     def from_folder(cls, model_dir, config: EngineConfig, verbose: bool = True) -> "Engine":

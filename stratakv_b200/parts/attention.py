@@ -8,6 +8,9 @@ sum of values in float; ``x += ctx.Wo^T`` (``src/layers/attention.cpp:153-342``,
 matrix ``[q | k | v]`` here, and the residual sum is the epilogue of the output
 projection.
 
+With ``cache_bits`` 4 keys and values are kept in 4 bits and a scale byte for each 16 numbers: one kernel rotates,
+quantises and appends, attention reads the codes (one or a few new tokens a sequence) or, for prompts, what they stand for.
+
 A spec may switch on further mechanisms (``parts/spec.py::AttentionSpec``): biases on the projections, values
 of another width than keys, an RMS norm on every value head before it is cached, a bias on the scores by the
 logarithm of the distance, and a gate per head on the output.  Such a mixer projects ``[q | k | v | gate]`` at
@@ -116,6 +119,10 @@ class PagedAttention(Mixer):
         super().__init__(spec, runtime)
         if spec.num_heads % spec.num_kv_heads != 0:
             raise ValueError("attention: heads must be a multiple of kv heads")
+        if spec.cache_bits not in (0, 4):
+            raise ValueError(f"attention: a cache of {spec.cache_bits} bits is not supported")
+        if spec.cache_bits and (spec.extended or runtime.dtype != torch.bfloat16):
+            raise ValueError("attention: a cache held in 4 bits serves plain attention in bfloat16")
         self.q_dim = spec.num_heads * spec.head_dim
         self.kv_dim = 0 if spec.shares_kv else spec.num_kv_heads * spec.head_dim
         self.v_dim = 0 if spec.shares_kv else spec.num_kv_heads * spec.value_dim
@@ -174,7 +181,7 @@ class PagedAttention(Mixer):
 
     @classmethod
     def cache_request(cls, spec):
-        kind = "kv_window" if spec.window > 0 else "kv"
+        kind = ("kv4" if spec.cache_bits == 4 else "kv") + ("_window" if spec.window > 0 else "")
         v_head_dim = spec.v_head_dim if spec.v_head_dim != spec.head_dim else 0
         return CacheRequest(kind, spec.num_kv_heads, spec.head_dim, spec.window, v_head_dim=v_head_dim)
 
@@ -331,7 +338,11 @@ class PagedAttention(Mixer):
         ops = rt.kernels(s.head_dim)
         n = h.shape[0]
         ctx = rt.workspace.get("attn_ctx", (n, self.q_dim), rt.dtype)
-        if (rt.dtype == torch.bfloat16 and n > 128 and s.head_dim in (64, 128) and torch.is_tensor(h)
+        if s.cache_bits:
+            qkv = rt.workspace.get("qkv", (n, self.q_dim + 2 * self.kv_dim), torch.float32)
+            ops.linear(h, self.w_qkv, qkv, _ops.MODE_STORE_F32)
+            self._attend_in_4_bits(step, qkv, ctx, cache_entry, writes_cache)
+        elif (rt.dtype == torch.bfloat16 and n > 128 and s.head_dim in (64, 128) and torch.is_tensor(h)
                 and hasattr(self.position, "fusion_table") and ops.has_linear_qkv_rope()):
             # many tokens: the projection's epilogue rotates queries and keys and writes the cache itself
             q = rt.workspace.get("q", (n, self.q_dim), rt.dtype)
@@ -371,6 +382,23 @@ class PagedAttention(Mixer):
         self.position.rotate_and_store(step, qkv, q, k_cache, v_cache, table, s.num_heads, s.num_kv_heads,
                                        s.head_dim, step.cache.block_size, writes_cache)
         self._attend_rotated(step, q, ctx, k_cache, v_cache, table)
+
+    def _attend_in_4_bits(self, step, qkv, ctx, cache_entry, writes_cache):
+        """The same over a cache held in 4 bits."""
+        s, rt = self.spec, self.rt
+        ops = rt.kernels(s.head_dim)
+        n, block_size = qkv.shape[0], step.cache.block_size
+        stored = step.cache.entry_storage(cache_entry)
+        cache = (stored["k"], stored["v"], stored["k_scale"], stored["v_scale"])
+        table = step.block_tables[step.cache.entry_group_index(cache_entry)]
+        q = rt.workspace.get("q", (n, self.q_dim), rt.dtype)
+        ops.append_kv4(qkv, self.position.fusion_table(step.max_ctx), step.positions, step.token_seq, table, q, *cache, s.num_heads,
+                       s.num_kv_heads, s.head_dim, block_size, writes_cache)
+        wanted = ops.attention_kv4_scratch(step.n_seqs, n, step.max_q_len, table.shape[1], s.num_heads, s.num_kv_heads, s.head_dim,
+                                           block_size, s.window)
+        scratch = rt.workspace.get("kv4_scratch", (wanted,), torch.uint8) if wanted else None
+        ops.attention_kv4(q, *cache, table, step.cu_q, step.ctx_after, ctx, step.max_q_len, s.num_heads, s.num_kv_heads, s.head_dim,
+                          block_size, s.scale, s.window, scratch)
 
     def _attend_rotated(self, step, q, ctx, k_cache, v_cache, table):
         """Attention of the step's rotated queries ``q`` over the cache, which holds the step's keys and values."""

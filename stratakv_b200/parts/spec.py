@@ -95,7 +95,8 @@ class AttentionSpec:
     attends over the cache entry that another layer's run wrote (its schedule entry names that entry and does
     not write it).  ``q_norm_weight`` / ``k_norm_weight`` (tensor names, ``[heads * head_dim]`` and
     ``[kv_heads * head_dim]``) with ``projection_norm_eps``: one RMS norm with that weight over ALL query heads
-    together, and one over all key heads, after the biases and before the heads are split."""
+    together, and one over all key heads, after the biases and before the heads are split.  ``cache_bits`` 4: keys and
+    values are kept in 4 bits and a scale byte for each 16 numbers (attention without any of the mechanisms above)."""
     hidden_size: int
     num_heads: int
     num_kv_heads: int
@@ -123,6 +124,7 @@ class AttentionSpec:
     q_norm_weight: Optional[str] = None
     k_norm_weight: Optional[str] = None
     projection_norm_eps: float = 0.0
+    cache_bits: int = 0              # 0: the compute dtype
 
     @property
     def value_dim(self) -> int:

@@ -22,7 +22,7 @@ MAX_NEW_TOKENS = 500          # runner.py:16
 
 def run(model_dir, prompts: Sequence[Sequence[int]], max_new_tokens: int = MAX_NEW_TOKENS, temp: float = 0.8,
         top_k: int = 40, top_p: float = 0.95, seed: int = 0, dtype: str = "bfloat16",
-        max_tokens: Optional[int] = None, ignore_eos: bool = False, engine=None):
+        max_tokens: Optional[int] = None, ignore_eos: bool = False, engine=None, cache_dtype: str = ""):
     """Generate for ``prompts`` (lists of token ids); returns ``(sequences, timings, engine)``."""
     from . import Engine, EngineConfig
     from .sampling import SamplingParams
@@ -31,7 +31,7 @@ def run(model_dir, prompts: Sequence[Sequence[int]], max_new_tokens: int = MAX_N
         block = 64
         need = sum(-(-(len(p) + max_new_tokens) // block) * block for p in prompts)
         engine = Engine.from_folder(model_dir, EngineConfig(max_tokens=max_tokens or need, dtype=dtype,
-                                                            block_size=block))
+                                                            block_size=block, cache_dtype=cache_dtype))
     output = engine.generate([list(p) for p in prompts], max_new_tokens,
                              SamplingParams(temp, top_k, top_p, seed), ignore_eos=ignore_eos)
     return output.sequences, output.timings, engine
@@ -47,6 +47,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--max-new-tokens", type=int, default=MAX_NEW_TOKENS)
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    parser.add_argument("--cache-dtype", default="", choices=["", "bfloat16", "float32", "int4"],
+                        help="what keys and values are kept in (default: the compute dtype)")
     parser.add_argument("--prompt-ids", type=int, nargs="+", help="the prompt as token ids")
     parser.add_argument("--prompt", help="the prompt as text (needs --tokenizer)")
     parser.add_argument("--tokenizer", help="folder of a tokenizer to encode --prompt and decode the output")
@@ -69,7 +71,7 @@ def main(argv=None) -> int:
     else:
         raise SystemExit("runner: give --prompt-ids or --prompt")
     sequences, timings, _ = run(options.model, [prompt_ids], options.max_new_tokens, options.temp, options.top_k,
-                                options.top_p, options.seed, options.dtype, ignore_eos=options.ignore_eos)
+                                options.top_p, options.seed, options.dtype, ignore_eos=options.ignore_eos, cache_dtype=options.cache_dtype)
     print(f"[TIMING] prefill_ms = {timings.prefill_ms:.3f}, decode_ms = {timings.decode_ms:.3f}, "
           f"decode_tokens = {timings.decode_tokens}, decode_tps = {timings.decode_tps:.1f}", file=sys.stderr)
     if tokenizer is not None:
