@@ -16,6 +16,8 @@
 
 #include "kv4.cuh"
 
+#include <type_traits>
+
 #if SKV_DTYPE == SKV_BF16
 
 namespace skv {
@@ -26,7 +28,24 @@ constexpr int KWORDS = FPAD / 32, VWORDS4 = FPAD / 64;      // words of eight co
 constexpr int KSTEP4 = FPAD / 16, OTILE4 = FPAD / 16;       // k16 steps of K Q^T; m16 tiles of V^T P^T
 // Scale bytes of a lane's words of a value: one where they lie in one group, one for two words or one each.
 constexpr int VGROUPS = FPAD == 192 ? 3 : FPAD == 256 ? 2 : 1, VWORDS_OF_GROUP = VWORDS4 / VGROUPS;
-constexpr int KV4_WARPS = 8;
+constexpr int KV4_WARPS = 8, KV4_SEQS = 1024;     // (sequences of a call)
+// A warp's chunk of CK keys (32, or 16 where a cache block is no multiple of 32) on its way: codes of keys and values, then their scales.
+constexpr int KROW = FHD / 2, SROW = FHD / 16, KV4_STAGES = FHD > 64 ? 2 : 3;
+template <int CK> constexpr int CHUNK_OF = CK * 2 * (KROW + SROW);
+template <int CK> constexpr int RING_OF = KV4_WARPS * KV4_STAGES * CHUNK_OF<CK>;
+
+// Index i of the sums over keys is key (i >> 1) + 4 (i & 1) of its eight: the four lanes that read values of one index then read four
+// neighbouring rows, which lie in different banks.  Keys are laid down in the order of the indices, where a row is whole pieces of 16
+// bytes (head sizes that are multiples of 32; of others a piece has the end of one row and the start of the next).
+constexpr bool KEYS_BY_INDEX = FHD % 32 == 0;
+constexpr int KREAD = FHD == 128 ? 4 : 2;         // words of a key a lane reads at once
+__device__ __forceinline__ int key_of_index(int i) { return (i & ~7) + ((i & 7) >> 1) + 4 * (i & 1); }
+__device__ __forceinline__ int index_of_key(int k) { return (k & ~7) + 2 * (k & 3) + ((k & 7) >> 2); }
+__device__ __forceinline__ void chunk_copy(uint32_t to, const uint8_t* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory");
+}
+// Where 16 bytes of a value's codes go (heads of 128: 64 bytes a row, of which two rows would share their banks).
+__device__ __forceinline__ int value_piece(int row, int piece) { return FHD == 128 ? piece ^ (row & 2) : piece; }
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -48,6 +67,24 @@ __device__ __forceinline__ float kv4_exp2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 // Probabilities are taken against a maximum that is raised when a score exceeds it by 2^8, and carry a factor 2^7: they stay
 // below 2^15 (a half ends at 65,504), and one 2^-21 of the largest still has all its 11 bits.
 constexpr float KV4_MARGIN = 8.0f, KV4_LIFT = 7.0f;
@@ -56,34 +93,139 @@ constexpr float KV4_MARGIN = 8.0f, KV4_LIFT = 7.0f;
 // NaN was among them, which must not get lost.
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 1.0f : kv4_exp2(m - top); }
 
-template <int NT>
-__global__ void __launch_bounds__(KV4_WARPS * 32)
+// How a step's work is cut.  An item is one key head of a sequence for one tile of rows; the chunks of all items, one item behind the other, are dealt
+// out to the warps in runs of equal length.  A run that begins or ends inside an item leaves a partial result, at most two a warp; an item that
+// one run holds whole is finished by it.  (Runs of blocks, whose warps take chunks in turn and add up in shared memory: 64 x 4,096 positions 79.6 us
+// against 73.9, 12 ragged sequences of 32 key heads 52.4 against 46.4.)
+struct Kv4Cut {
+    int n_seqs, num_heads, num_kv_heads, window, least;     // a run has at least `least` chunks
+    int most_positions, most_tiles;                         // what the call has room for
+};
+struct Kv4Share {
+    int q_begin, q_len, ctx, tiles, first_chunk, chunks;    // chunks of an item
+    __device__ __forceinline__ int all(const Kv4Cut& cut) const { return chunks * cut.num_kv_heads * tiles; }
+};
+template <int ROWS, int CK>
+__device__ __forceinline__ Kv4Share kv4_share(const Kv4Cut& cut, const int* cu_q, const int* ctx_after, int seq) {
+    Kv4Share s = {};
+    if (seq >= cut.n_seqs) return s;
+    s.q_begin = cu_q[seq];
+    s.q_len = cu_q[seq + 1] - s.q_begin;
+    s.ctx = min(ctx_after[seq], cut.most_positions);
+    s.tiles = min((s.q_len * (cut.num_heads / cut.num_kv_heads) + ROWS - 1) / ROWS, cut.most_tiles);
+    s.first_chunk = cut.window > 0 ? max(0, s.ctx - s.q_len - cut.window + 1) / CK : 0;
+    s.chunks = s.q_len > 0 ? (s.ctx + CK - 1) / CK - s.first_chunk : 0;
+    return s;
+}
+
+template <int NT, int CK>
+__global__ void __launch_bounds__(KV4_WARPS * 32, NT == 1 && FHD <= 128 ? 2 : 1)
 kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes,
                      const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale, const int* __restrict__ block_table,
                      int table_width, const int* __restrict__ cu_q, const int* __restrict__ ctx_after, __nv_bfloat16* __restrict__ out,
-                     float* __restrict__ partial_o, float* __restrict__ partial_ml, int num_heads, int num_kv_heads, int block_size,
-                     float scale, int window, int splits, int row_tiles) {
-    extern __shared__ float merge4[];                 // [warps][8 NT][FHD + 2]
-    constexpr int ROWS = 8 * NT, PITCH = FHD + 2;
+                     float4* __restrict__ partial_o, float2* __restrict__ partial_ml, const Kv4Cut cut, int block_size, float scale,
+                     uint32_t chunks_magic, uint32_t ones) {
+    extern __shared__ __align__(16) uint8_t kv4_smem[];
+    __shared__ int upto[KV4_SEQS], warp_all[KV4_WARPS];     // chunks up to and with a sequence; of a warp's sequences
+    constexpr int ROWS = 8 * NT;
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int seq = blockIdx.x, kv_head = blockIdx.y / row_tiles, row0 = (blockIdx.y - kv_head * row_tiles) * ROWS, split = blockIdx.z;
-    const int group = num_heads / num_kv_heads;
-    const int q_begin = cu_q[seq], q_len = cu_q[seq + 1] - q_begin, rows = q_len * group;
-    if (row0 >= rows) return;
-    const int ctx = ctx_after[seq], before = ctx - q_len;
+    const int num_heads = cut.num_heads, num_kv_heads = cut.num_kv_heads, window = cut.window, group = num_heads / num_kv_heads;
+    int total = 0;
+    for (int s0 = 0; s0 < cut.n_seqs; s0 += KV4_WARPS * 32) {
+        int sum = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, s0 + threadIdx.x).all(cut);
+#pragma unroll
+        for (int o2 = 1; o2 < 32; o2 *= 2) {
+            const int before = __shfl_up_sync(0xffffffffu, sum, o2);
+            if (lane >= o2) sum += before;
+        }
+        if (lane == 31) warp_all[warp] = sum;
+        __syncthreads();
+        for (int w = 0; w < KV4_WARPS; ++w) {
+            const int v = warp_all[w];
+            if (w < warp) sum += v;
+        }
+        if (s0 + threadIdx.x < cut.n_seqs) upto[s0 + threadIdx.x] = total + sum;
+        __syncthreads();
+        total = upto[min(s0 + KV4_WARPS * 32, cut.n_seqs) - 1];
+    }
+    const int workers = (int)gridDim.x * KV4_WARPS, run = max(cut.least, (total + workers - 1) / workers);
+    const int worker = blockIdx.x + gridDim.x * warp;       // (runs that follow each other lie on different SMs)
+    const long long run_begin = (long long)worker * run;
+    if (run_begin >= total) return;
+    const int run_end = (int)min((long long)total, run_begin + run);
+    int seq = 0;                                            // the first whose chunks reach beyond run_begin
+    for (int step = KV4_SEQS / 2; step > 0; step /= 2)
+        if (seq + step <= cut.n_seqs && upto[seq + step - 1] <= (int)run_begin) seq += step;
+
+    for (int done = (int)run_begin; done < run_end;) {
+    while (upto[seq] <= done) ++seq;                        // (sequences without tokens have no chunks)
+    const Kv4Share share = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, seq);
+    const int q_begin = share.q_begin, q_len = share.q_len, tiles = share.tiles;
+    const int in_seq = done - (seq ? upto[seq - 1] : 0), item = in_seq / share.chunks, from = in_seq - item * share.chunks;
+    const int count = min(run_end - done, share.chunks - from), kv_head = item / tiles;
+    const bool whole = count == share.chunks;
+    const size_t slot = (size_t)2 * worker + (done != (int)run_begin);
+    done += count;
+    const int row0 = (item - kv_head * tiles) * ROWS, rows = q_len * group, before = share.ctx - q_len;
     const int last_query = min(rows, row0 + ROWS) - 1;
-    const int end = before + last_query / group + 1;                        // keys that any row of the block sees: lo .. end - 1
-    const int lo = window > 0 ? max(0, before + row0 / group - window + 1) : 0;
-    const int first_group = lo >> 4, end_group = (end + 15) >> 4, per_split = (end_group - first_group + splits - 1) / splits;
-    const int my_first = first_group + split * per_split, my_end = min(end_group, my_first + per_split);
+    const int end = before + last_query / group + 1;                        // keys that any row of the tile sees lie before it
+    const int my_first = share.first_chunk + from, my_end = min(my_first + count, (end + CK - 1) / CK);
     const int* table = block_table + (size_t)seq * table_width;
+
+    // Copies of a chunk: pieces of 16 bytes, a lane one after the other.
+    constexpr int CHUNK_BYTES = CHUNK_OF<CK>, PIECES = FHD % 32 ? 1 : FHD / 32;      // (of a row)
+    const uint32_t ring = smem_u32(kv4_smem) + (uint32_t)(warp * KV4_STAGES * CHUNK_BYTES);
+    const uint32_t block_bytes = (uint32_t)num_kv_heads * block_size * KROW;
+    const uint8_t* k_from = k_codes + (size_t)kv_head * block_size * KROW + 16 * lane;
+    const uint8_t* v_from = v_codes + (size_t)kv_head * block_size * KROW + 16 * lane;
+    constexpr int SCALE_PIECES = CK * SROW / 16;
+    const uint8_t* s_from = (lane < SCALE_PIECES || SCALE_PIECES > 16 ? k_scale + 16 * lane : v_scale + 16 * (lane - SCALE_PIECES)) + (size_t)kv_head * block_size * SROW;
+    const uint32_t k_to = KEYS_BY_INDEX ? index_of_key(lane / PIECES) * KROW + 16 * (lane % PIECES) : 16 * lane;
+    const uint32_t v_to = CK * KROW + (KEYS_BY_INDEX ? lane / PIECES * KROW + 16 * value_piece(lane / PIECES, lane % PIECES) : 16 * lane);
+    auto block_of = [&](int chunk) { return chunks_magic ? (int)__umulhi((uint32_t)chunk, chunks_magic) : chunk; };
+    auto fetch = [&](int chunk, int block, uint32_t to) {
+        const uint32_t inside = (uint32_t)(chunk * CK - block_of(chunk) * block_size);
+        const uint8_t* kc = k_from + ((size_t)(uint32_t)block * block_bytes + inside * KROW);
+        const uint8_t* vc = v_from + ((size_t)(uint32_t)block * block_bytes + inside * KROW);
+        const uint8_t* sc = s_from + ((size_t)(uint32_t)block * (block_bytes / 8) + inside * SROW);
+#pragma unroll
+        for (int u = 0; u < CK * KROW / 16; u += 32) {
+            if (CK * KROW / 16 % 32 && u + lane >= CK * KROW / 16) break;
+            if (!KEYS_BY_INDEX || (32 % PIECES == 0 && 32 / PIECES % 8 == 0)) {
+                chunk_copy(to + k_to + 16 * u, kc + 16 * u);         // (whole groups of eight keys further)
+                chunk_copy(to + v_to + 16 * u, vc + 16 * u);
+            } else {
+                const int key = (u + lane) / PIECES, piece = u + lane - key * PIECES;
+                chunk_copy(to + index_of_key(key) * KROW + 16 * piece, kc + 16 * u);
+                chunk_copy(to + CK * KROW + key * KROW + 16 * piece, vc + 16 * u);
+            }
+        }
+        const uint32_t scales_to = to + 2 * CK * KROW + 16 * lane;
+        if (SCALE_PIECES <= 16) {                     // both sorts at once
+            if (lane < 2 * SCALE_PIECES) chunk_copy(scales_to, sc);
+        } else if (lane < SCALE_PIECES) {
+            chunk_copy(scales_to, sc);
+            chunk_copy(scales_to + CK * SROW, v_scale + (sc - k_scale));
+        }
+    };
+
+    int ahead = my_first;                             // the chunk that is fetched next, and its block
+    auto entry = [&](int chunk) { return chunk < my_end ? table[block_of(chunk)] : 0; };
+    int block = entry(ahead);
+#pragma unroll
+    for (int st = 0; st < KV4_STAGES - 1; ++st) {
+        const int following = entry(ahead + 1);
+        if (ahead < my_end) fetch(ahead, block, ring + st * CHUNK_BYTES);
+        ring_commit();
+        ++ahead;
+        block = following;
+    }
 
     // Queries: lane (g, t) has a quarter of row g of each tile of eight; word j's codes p and p + 4 meet numbers 8j + p and 8j + p + 4.
     uint32_t qb[NT][KSTEP4][2];
-    float factor[NT][2];                              // of rows 2t and 2t + 1: scale * log2 e * the power of two taken off the query
-    int position[NT][2];                              // and where they sit (-1: no such row)
+    float2 factor[NT];                              // of rows 2t and 2t + 1: scale * log2 e * the power of two taken off the query
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = row0 + 8 * n + g;
@@ -122,13 +264,7 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
             qb[n][2 * j + 1][0] = pack_half(x[2], x[6]); qb[n][2 * j + 1][1] = pack_half(x[3], x[7]);
         }
         const float up = scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + power) << 23);
-        factor[n][0] = __shfl_sync(0xffffffffu, up, 8 * t);
-        factor[n][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int of = row0 + 8 * n + 2 * t + c;
-            position[n][c] = of < rows ? before + of / group : -1;
-        }
+        factor[n] = make_float2(__shfl_sync(0xffffffffu, up, 8 * t), __shfl_sync(0xffffffffu, up, 8 * t + 4));
     }
 
     float o[OTILE4][NT][4];
@@ -136,245 +272,405 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     for (int j = 0; j < OTILE4; ++j)
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
-    float most[NT][2], sum[NT][2];
+    float2 lift[NT], sum[NT];                         // KV4_LIFT less the maximum in use of rows 2t and 2t + 1; their sums
 #pragma unroll
-    for (int n = 0; n < NT; ++n) { most[n][0] = most[n][1] = -INFINITY; sum[n][0] = sum[n][1] = 0.0f; }
+    for (int n = 0; n < NT; ++n) { lift[n] = make_float2(INFINITY, INFINITY); sum[n] = make_float2(0.0f, 0.0f); }
 
-    for (int at = my_first + warp; at < my_end; at += KV4_WARPS) {
-        const int j0 = at << 4;
-        const size_t row = ((size_t)table[j0 / block_size] * num_kv_heads + kv_head) * block_size + j0 % block_size;
-        const int live = min(16, ctx - j0);           // keys behind them hold what earlier users of the block left
-
-        // codes and scales of keys g and g + 8, of values 2t, 2t + 1, 2t + 8 and 2t + 9
-        uint32_t kw[2][KWORDS], ks[2][KWORDS / 2], vw[4][VWORDS4], vs[4][VGROUPS];
+    // One chunk.  MASKED: some row of the block does not see all of its keys.
+    const uint32_t k_lane = (KEYS_BY_INDEX ? g : key_of_index(g)) * KROW + t * (FPAD / 8);
+    const uint32_t ks_lane = 2 * CK * KROW + key_of_index(g) * SROW + t * (FPAD / 64), vs_lane = 2 * CK * KROW + CK * SROW + t * SROW;
+    auto attend = [&](auto masked_, int j0, const uint8_t* tile) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        constexpr int HALVES = CK / 16;
+        int position[NT][2];                          // where rows 2t and 2t + 1 sit (-1: no such row)
+        if (MASKED) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int key = g + 8 * i;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < KWORDS; j += 2) {
-                const int d = t * (FPAD / 4) + 8 * j;
-                const bool there = d < FHD && key < live;
-                const uint2 w = there ? *(const uint2*)(k_codes + (row + key) * (FHD / 2) + d / 2) : make_uint2(0u, 0u);
-                kw[i][j] = w.x; kw[i][j + 1] = w.y;
-                ks[i][j / 2] = there ? k_scale[(row + key) * (FHD / 16) + d / 16] : 0u;
-            }
+                for (int c = 0; c < 2; ++c) {
+                    const int r = row0 + 8 * n + 2 * t + c;
+                    position[n][c] = r < rows ? before + r / group : -1;
+                }
+        }
+        // S^T: keys of indices g, g + 8 by rows 2t, 2t + 1.  Two sums take turns: an instruction that adds to the one before it would wait for it.
+        float s[HALVES][NT][4], other[HALVES][NT][4];
+        uint32_t kw[HALVES][2][KWORDS];
+#pragma unroll
+        for (int h16 = 0; h16 < HALVES; ++h16) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[h16][n][c] = other[h16][n][c] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < KWORDS; j += KREAD) {
+                    const bool there = FHD == FPAD || t * (FPAD / 4) + 8 * j < FHD;
+                    const uint8_t* from = tile + k_lane + (16 * h16 + 8 * i) * KROW + 4 * j;
+                    if (KREAD == 4) {
+                        const uint4 w = *(const uint4*)from;
+                        kw[h16][i][j] = w.x; kw[h16][i][j + 1] = w.y; kw[h16][i][j + 2] = w.z; kw[h16][i][j + KREAD - 1] = w.w;
+                    } else {
+                        const uint2 w = there ? *(const uint2*)from : make_uint2(0u, 0u);
+                        kw[h16][i][j] = w.x; kw[h16][i][j + 1] = w.y;
+                    }
+                }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+        for (int j = 0; j < KWORDS; j += 2)
 #pragma unroll
-            for (int j = 0; j < VWORDS4; ++j) {
-                const int d = g * (FPAD / 8) + 8 * j;
-                const bool there = d < FHD && key < live;
-                vw[i][j] = there ? *(const uint32_t*)(v_codes + (row + key) * (FHD / 2) + d / 2) : 0u;
-                if (j % VWORDS_OF_GROUP == 0) vs[i][j / VWORDS_OF_GROUP] = there ? v_scale[(row + key) * (FHD / 16) + d / 16] : 0u;
-            }
-        }
-
-        // S^T: keys g, g + 8 by rows 2t, 2t + 1
-        float s[NT][4];
+            for (int h16 = 0; h16 < HALVES; ++h16) {
+                const bool there = FHD == FPAD || t * (FPAD / 4) + 8 * j < FHD;
+                Kv4Scale of[2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+                for (int i = 0; i < 2; ++i)
+                    of[i] = kv4_pair_of_scales((there ? (uint32_t)tile[ks_lane + (16 * h16 + 8 * i) * SROW + j / 2] : 0u) * 0x00800080u);
 #pragma unroll
-        for (int j = 0; j < KWORDS; ++j) {
-            uint32_t a[2][4];
+                for (int w = 0; w < 2; ++w) {
+                    uint32_t a[2][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t h = ks[i][j / 2] * 0x00800080u, off = kv4_offset(h);
-                kv4_spread(kw[i][j], a[i]);
+                    for (int i = 0; i < 2; ++i) kv4_unpack(kw[h16][i][j + w], of[i], ones, a[i]);
 #pragma unroll
-                for (int p = 0; p < 4; ++p) a[i][p] = kv4_value(a[i][p], h, off);
+                    for (int n = 0; n < NT; ++n) {
+                        mma_f16_16816(s[h16][n], a[0][0], a[1][0], a[0][1], a[1][1], qb[n][2 * (j + w)][0], qb[n][2 * (j + w)][1]);
+                        mma_f16_16816(other[h16][n], a[0][2], a[1][2], a[0][3], a[1][3], qb[n][2 * (j + w) + 1][0], qb[n][2 * (j + w) + 1][1]);
+                    }
+                }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma_f16_16816(s[n], a[0][0], a[1][0], a[0][1], a[1][1], qb[n][2 * j][0], qb[n][2 * j][1]);
-                mma_f16_16816(s[n], a[0][2], a[1][2], a[0][3], a[1][3], qb[n][2 * j + 1][0], qb[n][2 * j + 1][1]);
-            }
-        }
-        bool raise = false;
+        for (int h16 = 0; h16 < HALVES; ++h16)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int key = j0 + g + 8 * (c >> 1), pos = position[n][c & 1];
-                const bool seen = key <= pos && (window == 0 || key > pos - window);
-                s[n][c] = seen ? s[n][c] * factor[n][c & 1] : -INFINITY;
-                raise = raise || s[n][c] > most[n][c & 1] + KV4_MARGIN;
-            }
-        if (__any_sync(0xffffffffu, raise)) {
+                for (int c = 0; c < 4; c += 2) {
+                    const float2 v = add2(make_float2(s[h16][n][c], s[h16][n][c + 1]), make_float2(other[h16][n][c], other[h16][n][c + 1]));
+                    s[h16][n][c] = v.x; s[h16][n][c + 1] = v.y;
+                }
+        auto sees = [&](int h16, int n, int c) {
+            const int key = j0 + 16 * h16 + key_of_index(g) + 8 * (c >> 1), pos = position[n][c & 1];
+            return key <= pos && (window == 0 || key > pos - window);
+        };
+        // Scores in units of log2, above the maximum in use and with its lift.  (Nothing seen before: +infinity, which raises it.)
+        float y[HALVES][NT][4];
+        auto place = [&] {
+#pragma unroll
+            for (int h16 = 0; h16 < HALVES; ++h16)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        const float2 v = fma2(make_float2(s[h16][n][c], s[h16][n][c + 1]), factor[n], lift[n]);
+                        y[h16][n][c] = !MASKED || sees(h16, n, c) ? v.x : -INFINITY;
+                        y[h16][n][c + 1] = !MASKED || sees(h16, n, c + 1) ? v.y : -INFINITY;
+                    }
+        };
+        place();
+        float top = -INFINITY;
+#pragma unroll
+        for (int h16 = 0; h16 < HALVES; ++h16)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) top = max3(max3(top, y[h16][n][0], y[h16][n][1]), y[h16][n][2], y[h16][n][3]);
+        if (__any_sync(0xffffffffu, top > KV4_MARGIN + KV4_LIFT)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float by[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float m = fmaxf(s[n][c], s[n][c + 2]);
+                    const float f = c ? factor[n].y : factor[n].x;
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int h16 = 0; h16 < HALVES; ++h16)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) m = fmaxf(m, !MASKED || sees(h16, n, c + i) ? s[h16][n][c + i] * f : -INFINITY);
 #pragma unroll
                     for (int o2 = 4; o2 < 32; o2 *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
-                    m = fmaxf(m, most[n][c]);
-                    by[c] = m == most[n][c] ? 1.0f : kv4_exp2(most[n][c] - m);       // (0 if nothing was seen before)
-                    most[n][c] = m;
-                    sum[n][c] *= by[c];
+                    const float was = c ? lift[n].y : lift[n].x, now = fminf(was, KV4_LIFT - m);
+                    by[c] = now == was ? 1.0f : kv4_exp2(now - was);                 // (0 if nothing was seen before)
+                    if (c) { lift[n].y = now; sum[n].y *= by[1]; } else { lift[n].x = now; sum[n].x *= by[0]; }
                 }
 #pragma unroll
                 for (int j = 0; j < OTILE4; ++j) { o[j][n][0] *= by[0]; o[j][n][1] *= by[1]; o[j][n][2] *= by[0]; o[j][n][3] *= by[1]; }
             }
+            place();
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[HALVES][NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float p[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float m = most[n][c & 1];
-                p[c] = kv4_exp2(s[n][c] - (m == -INFINITY ? 0.0f : m) + KV4_LIFT);
-                sum[n][c & 1] += p[c];
-            }
-            pb[n][0] = turn_8x8(pack_half(p[0], p[1]));
-            pb[n][1] = turn_8x8(pack_half(p[2], p[3]));
-        }
-        // A NaN among the values reaches the rows that see its key alone: times a masked key's zero it would reach all.
-        uint32_t spoiled = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < VGROUPS; ++j)
-                if (vs[i][j] > KV4_LARGEST) { spoiled |= 1u << (4 * j + i); vs[i][j] = 0u; }
-        // O^T += V^T P^T
-#pragma unroll
-        for (int j = 0; j < VWORDS4; ++j) {
-            const int of = j / VWORDS_OF_GROUP;
-            const uint32_t h01 = (vs[0][of] | vs[1][of] << 16) << 7, h89 = (vs[2][of] | vs[3][of] << 16) << 7;
-            const uint32_t off01 = kv4_offset(h01), off89 = kv4_offset(h89);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t x[4], y[4];
-                kv4_spread(__byte_perm(vw[0][j], vw[1][j], half ? 0x7632 : 0x5410), x);
-                kv4_spread(__byte_perm(vw[2][j], vw[3][j], half ? 0x7632 : 0x5410), y);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) { x[p] = kv4_value(x[p], h01, off01); y[p] = kv4_value(y[p], h89, off89); }
-#pragma unroll
-                for (int p = 0; p < 4; p += 2)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        mma_f16_16816(o[4 * j + 2 * half + p / 2][n], x[p], x[p + 1], y[p], y[p + 1], pb[n][0], pb[n][1]);
-            }
-        }
-        if (__any_sync(0xffffffffu, spoiled != 0u)) {
-            // how many NaN a row sees in a group of numbers: a product of ones
+        for (int h16 = 0; h16 < HALVES; ++h16)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float sees[4];
+                float p[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int key = j0 + g + 8 * (c >> 1), pos = position[n][c & 1];
-                    sees[c] = key <= pos && (window == 0 || key > pos - window) ? 1.0f : 0.0f;
-                }
-                const uint32_t b0 = turn_8x8(pack_half(sees[0], sees[1])), b1 = turn_8x8(pack_half(sees[2], sees[3]));
+                for (int c = 0; c < 4; ++c) p[c] = kv4_exp2(y[h16][n][c]);
+                sum[n] = add2(sum[n], add2(make_float2(p[0], p[1]), make_float2(p[2], p[3])));
+                pb[h16][n][0] = turn_8x8(pack_half(p[0], p[1]));
+                pb[h16][n][1] = turn_8x8(pack_half(p[2], p[3]));
+            }
+#pragma unroll
+        for (int h16 = 0; h16 < HALVES; ++h16) {
+            // Scales of the values of indices 2t, 2t + 1, 2t + 8 and 2t + 9: keys t, t + 4, t + 8 and t + 12.
+            uint32_t vs[4][VGROUPS], spoiled = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < VGROUPS; ++j) {
-                    const uint32_t bits = spoiled >> (4 * j);
-                    const uint32_t a01 = pack_half(bits & 1u ? 1.0f : 0.0f, bits & 2u ? 1.0f : 0.0f);
-                    const uint32_t a89 = pack_half(bits & 4u ? 1.0f : 0.0f, bits & 8u ? 1.0f : 0.0f);
-                    float count[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16_16816(count, a01, a01, a89, a89, b0, b1);
+                    const int d = g * (FPAD / 8) + 8 * VWORDS_OF_GROUP * j;
+                    vs[i][j] = FHD == FPAD || d < FHD ? tile[vs_lane + (16 * h16 + 4 * i) * SROW + d / 16] : 0u;
+                    if (MASKED) {
+                        // Rows behind the sequence hold what earlier users of the block left.  A NaN among the values reaches the rows that
+                        // see its key alone: times a masked key's zero it would reach all.
+                        if (j0 + 16 * h16 + t + 4 * i >= end) vs[i][j] = 0u;
+                        if (vs[i][j] > KV4_LARGEST) { spoiled |= 1u << (4 * j + i); vs[i][j] = 0u; }
+                    }
+                }
+            // O^T += V^T P^T
+            uint32_t words[4][VWORDS4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (count[c] > 0.0f) {
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t* from = tile + CK * KROW + (16 * h16 + t + 4 * i) * KROW;
 #pragma unroll
-                            for (int w = 0; w < 4 * VWORDS_OF_GROUP; ++w) o[4 * VWORDS_OF_GROUP * j + w][n][c] = NAN;
+                for (int j = 0; j < VWORDS4; ++j) {
+                    const int d = g * (FPAD / 8) + 8 * j;
+                    if (FHD == 128) {
+                        if (j == 0) {                  // (both words lie in one piece of 16 bytes)
+                            const uint2 w = *(const uint2*)(from + 16 * value_piece(t, g / 2) + 8 * (g & 1));
+                            words[i][0] = w.x; words[i][VWORDS4 - 1] = w.y;
                         }
+                    } else {
+                        words[i][j] = FHD == FPAD || d < FHD ? *(const uint32_t*)(from + d / 2) : 0u;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VWORDS4; ++j) {
+                const int of = j / VWORDS_OF_GROUP;
+                const Kv4Scale of01 = kv4_pair_of_scales(vs[1][of] * 0x00800000u + vs[0][of] * 0x80u);
+                const Kv4Scale of89 = kv4_pair_of_scales(vs[3][of] * 0x00800000u + vs[2][of] * 0x80u);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t x[4], z[4];
+                    kv4_unpack(__byte_perm(words[0][j], words[1][j], half ? 0x7632 : 0x5410), of01, ones, x);
+                    kv4_unpack(__byte_perm(words[2][j], words[3][j], half ? 0x7632 : 0x5410), of89, ones, z);
+#pragma unroll
+                    for (int p = 0; p < 4; p += 2)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            mma_f16_16816(o[4 * j + 2 * half + p / 2][n], x[p], x[p + 1], z[p], z[p + 1], pb[h16][n][0], pb[h16][n][1]);
+                }
+            }
+            if (MASKED && __any_sync(0xffffffffu, spoiled != 0u)) {
+                // how many NaN a row sees in a group of numbers: a product of ones
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t b0 = turn_8x8(pack_half(sees(h16, n, 0) ? 1.0f : 0.0f, sees(h16, n, 1) ? 1.0f : 0.0f));
+                    const uint32_t b1 = turn_8x8(pack_half(sees(h16, n, 2) ? 1.0f : 0.0f, sees(h16, n, 3) ? 1.0f : 0.0f));
+#pragma unroll
+                    for (int j = 0; j < VGROUPS; ++j) {
+                        const uint32_t bits = spoiled >> (4 * j);
+                        const uint32_t a01 = pack_half(bits & 1u ? 1.0f : 0.0f, bits & 2u ? 1.0f : 0.0f);
+                        const uint32_t a89 = pack_half(bits & 4u ? 1.0f : 0.0f, bits & 8u ? 1.0f : 0.0f);
+                        float count[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_f16_16816(count, a01, a01, a89, a89, b0, b1);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (count[c] > 0.0f) {
+#pragma unroll
+                                for (int w = 0; w < 4 * VWORDS_OF_GROUP; ++w) o[4 * VWORDS_OF_GROUP * j + w][n][c] = NAN;
+                            }
+                    }
                 }
             }
         }
+    };
+
+    // every row of the block sees keys all_from .. all_to - 1
+    const int all_to = before + row0 / group + 1, all_from = window > 0 ? max(0, before + last_query / group - window + 1) : 0;
+    int stage = 0, free_stage = KV4_STAGES - 1;
+    for (int at = my_first; at < my_end; ++at) {
+        ring_wait<KV4_STAGES - 2>();
+        __syncwarp();                                 // the chunk is here for all lanes, and all have left the one before
+        const int following = entry(ahead + 1);
+        if (ahead < my_end) fetch(ahead, block, ring + free_stage * CHUNK_BYTES);
+        ring_commit();
+        ++ahead;
+        block = following;
+        const int j0 = at * CK;
+        const uint8_t* tile = kv4_smem + (warp * KV4_STAGES + stage) * CHUNK_BYTES;
+        if (j0 + CK <= all_to && j0 >= all_from) attend(std::false_type{}, j0, tile);
+        else attend(std::true_type{}, j0, tile);
+        free_stage = stage;
+        stage = stage + 1 == KV4_STAGES ? 0 : stage + 1;
     }
-    // merge the warps
-    float* mine = merge4 + (size_t)warp * ROWS * PITCH;
+    ring_wait<0>();
+    __syncwarp();                                     // (the next item's chunks go where these were)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int o2 = 4; o2 < 32; o2 *= 2) {
+            sum[n].x += __shfl_xor_sync(0xffffffffu, sum[n].x, o2);
+            sum[n].y += __shfl_xor_sync(0xffffffffu, sum[n].y, o2);
+        }
+        if (!whole) {
+            // left as they lie in the registers: a lane's four numbers of a tile
 #pragma unroll
-            for (int o2 = 4; o2 < 32; o2 *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], o2);
-            float* to = mine + (8 * n + 2 * t + c) * PITCH;
-#pragma unroll
-            for (int j = 0; j < OTILE4; ++j) {
-                const int d = g * (FPAD / 8) + 2 * j;
-                if (d < FHD) *(float2*)(to + d) = make_float2(o[j][n][c], o[j][n][c + 2]);
+            for (int j = 0; j < OTILE4; ++j)
+                partial_o[((slot * NT + n) * OTILE4 + j) * 32 + lane] = make_float4(o[j][n][0], o[j][n][1], o[j][n][2], o[j][n][3]);
+            if (g == 0) {
+                partial_ml[slot * ROWS + 8 * n + 2 * t] = make_float2(-lift[n].x, sum[n].x);
+                partial_ml[slot * ROWS + 8 * n + 2 * t + 1] = make_float2(-lift[n].y, sum[n].y);
             }
-            if (g == 0) { to[FHD] = most[n][c]; to[FHD + 1] = sum[n][c]; }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int r = row0 + 8 * n + 2 * t + c;
+                if (r >= rows) continue;
+                __nv_bfloat16* to = out + ((size_t)(q_begin + r / group) * num_heads + kv_head * group + r % group) * FHD;
+                const float by = 1.0f / (c ? sum[n].y : sum[n].x);
+#pragma unroll
+                for (int j = 0; j < OTILE4; ++j) {
+                    const int d = g * (FPAD / 8) + 2 * j;
+                    if (d < FHD) *(__nv_bfloat162*)(to + d) = __floats2bfloat162_rn(o[j][n][c] * by, o[j][n][c + 2] * by);
+                }
+            }
         }
     }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < ROWS * FHD; idx += blockDim.x) {
-        const int r = idx / FHD, d = idx - r * FHD;
-        if (row0 + r >= rows) break;
-        float m = -INFINITY;
-        for (int w = 0; w < KV4_WARPS; ++w) m = fmaxf(m, merge4[((size_t)w * ROWS + r) * PITCH + FHD]);
-        float total = 0.0f, l = 0.0f;
-        for (int w = 0; w < KV4_WARPS; ++w) {
-            const float* from = merge4 + ((size_t)w * ROWS + r) * PITCH;
-            const float weight = part_weight(from[FHD], m);
-            total += weight * from[d];
-            l += weight * from[FHD + 1];
-        }
-        const size_t item = (size_t)(q_begin + (row0 + r) / group) * num_heads + kv_head * group + (row0 + r) % group;
-        if (splits == 1) {
-            out[item * FHD + d] = __float2bfloat16_rn(total / l);
-        } else {
-            partial_o[(item * splits + split) * FHD + d] = total;
-            if (d == 0) { partial_ml[2 * (item * splits + split)] = m; partial_ml[2 * (item * splits + split) + 1] = l; }
-        }
     }
 }
 
-constexpr int KV4_COMBINE_THREADS = (FHD + 31) / 32 * 32;
-
-__global__ void __launch_bounds__(KV4_COMBINE_THREADS)
-kv4_combine_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, const int* __restrict__ cu_q,
-                   __nv_bfloat16* __restrict__ out, int n_seqs, int num_heads, int splits) {
+// The partial results of an item, brought to their common maximum and added up in their order: a warp has a tile of 16 numbers.  SPREAD: eight warps have
+// it, partial results in turn, for few items of many.
+template <int NT, int CK, bool SPREAD>
+__global__ void __launch_bounds__(KV4_WARPS * 32)
+kv4_merge_kernel(const float4* __restrict__ partial_o, const float4* __restrict__ partial_ml, const int* __restrict__ cu_q,
+                 const int* __restrict__ ctx_after, __nv_bfloat16* __restrict__ out, const Kv4Cut cut, int workers) {
+    constexpr int ROWS = 8 * NT, AHEAD = 8;
+    __shared__ float4 shared_o[KV4_WARPS][32], shared_ml[KV4_WARPS][32];
+    __shared__ int sums[2][KV4_WARPS];
     pdl_launch_dependents();
     pdl_wait();
-    const size_t item = blockIdx.x;
-    const int d = threadIdx.x;
-    if (d >= FHD || blockIdx.x >= cu_q[n_seqs] * num_heads) return;     // (rows behind the last sequence stay as they are)
-    const float* ml = partial_ml + 2 * item * splits;
-    float m = -INFINITY, total = 0.0f, l = 0.0f;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[2 * s]);
-    for (int s = 0; s < splits; ++s) {
-        const float weight = part_weight(ml[2 * s], m);
-        total += weight * partial_o[(item * splits + s) * FHD + d];
-        l += weight * ml[2 * s + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int of_seq = cut.num_kv_heads * cut.most_tiles, seq = blockIdx.x / of_seq, item = blockIdx.x - seq * of_seq;
+    const int kv_head = item / cut.most_tiles, at_tile = item - kv_head * cut.most_tiles, group = cut.num_heads / cut.num_kv_heads;
+    const Kv4Share share = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, seq);
+    int total = 0, base = 0;                          // chunks of all sequences, and of those before this one
+    for (int s = threadIdx.x; s < cut.n_seqs; s += KV4_WARPS * 32) {
+        const int all = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, s).all(cut);
+        total += all;
+        if (s < seq) base += all;
     }
-    out[item * FHD + d] = __float2bfloat16_rn(total / l);
+    total = __reduce_add_sync(0xffffffffu, total);
+    base = __reduce_add_sync(0xffffffffu, base);
+    if (lane == 0) { sums[0][warp] = total; sums[1][warp] = base; }
+    __syncthreads();
+    if (at_tile >= share.tiles || share.chunks == 0) return;
+    total = base = 0;
+#pragma unroll
+    for (int w = 0; w < KV4_WARPS; ++w) { total += sums[0][w]; base += sums[1][w]; }
+    const int run = max(cut.least, (total + workers - 1) / workers);
+    const int begin = base + (kv_head * share.tiles + at_tile) * share.chunks, first = begin / run, parts = (begin + share.chunks - 1) / run - first + 1;
+    if (parts == 1) return;                           // finished by the warp that had it
+    auto slot_of = [&](int p) { return (size_t)2 * (first + p) + (p == 0 && begin != first * run); };
+    for (int tile = SPREAD ? blockIdx.y : warp; tile < OTILE4 * NT; tile += SPREAD ? OTILE4 * NT : KV4_WARPS) {
+        const int n = tile / OTILE4, j = tile - n * OTILE4;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float2 top = make_float2(-INFINITY, -INFINITY), sum = make_float2(0.0f, 0.0f);
+        for (int p0 = SPREAD ? warp : 0; p0 < parts; p0 += AHEAD * (SPREAD ? KV4_WARPS : 1)) {
+            float4 o[AHEAD], ml[AHEAD];               // (maximum and sum of rows 2t and 2t + 1)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int p = p0 + u * (SPREAD ? KV4_WARPS : 1);
+                const size_t at = slot_of(p);
+                o[u] = p < parts ? partial_o[((at * NT + n) * OTILE4 + j) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                ml[u] = p < parts ? partial_ml[at * (ROWS / 2) + 4 * n + t] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+            }
+            float2 now = top;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) now = make_float2(fmaxf(now.x, ml[u].x), fmaxf(now.y, ml[u].z));
+            const float2 by = make_float2(part_weight(top.x, now.x), part_weight(top.y, now.y));
+            acc = make_float4(acc.x * by.x, acc.y * by.y, acc.z * by.x, acc.w * by.y);
+            sum = make_float2(sum.x * by.x, sum.y * by.y);
+            top = now;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const float a = part_weight(ml[u].x, now.x), b = part_weight(ml[u].z, now.y);
+                acc = make_float4(acc.x + o[u].x * a, acc.y + o[u].y * b, acc.z + o[u].z * a, acc.w + o[u].w * b);
+                sum = make_float2(sum.x + ml[u].y * a, sum.y + ml[u].w * b);
+            }
+        }
+        if (SPREAD) {
+            shared_o[warp][lane] = acc;
+            shared_ml[warp][lane] = make_float4(top.x, sum.x, top.y, sum.y);
+            __syncthreads();
+            if (warp != 0) return;
+            acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            sum = make_float2(0.0f, 0.0f);
+            for (int w = 0; w < KV4_WARPS; ++w) top = make_float2(fmaxf(top.x, shared_ml[w][lane].x), fmaxf(top.y, shared_ml[w][lane].z));
+            for (int w = 0; w < KV4_WARPS; ++w) {
+                const float4 v = shared_o[w][lane], ml = shared_ml[w][lane];
+                const float a = part_weight(ml.x, top.x), b = part_weight(ml.z, top.y);
+                acc = make_float4(acc.x + v.x * a, acc.y + v.y * b, acc.z + v.z * a, acc.w + v.w * b);
+                sum = make_float2(sum.x + ml.y * a, sum.y + ml.w * b);
+            }
+        }
+        const int d = g * (FPAD / 8) + 2 * j;
+        if (d >= FHD) continue;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = at_tile * ROWS + 8 * n + 2 * t + c;
+            if (r >= share.q_len * group) continue;
+            const float by = 1.0f / (c ? sum.y : sum.x);
+            *(__nv_bfloat162*)(out + ((size_t)(share.q_begin + r / group) * cut.num_heads + kv_head * group + r % group) * FHD + d) =
+                __floats2bfloat162_rn((c ? acc.y : acc.x) * by, (c ? acc.w : acc.z) * by);
+        }
+    }
 }
 
-static int kv4_row_tiles(int max_q_len, int group) { return max_q_len * group > 8 ? (max_q_len * group + 15) / 16 : 1; }
+// How a step of these sizes is cut: as many runs as warps fit the GPU, and how many partial results an item has at most.
+struct Kv4Plan {
+    Kv4Cut cut;
+    int chunk, tiles_of_8, blocks;
+    long long items, chunks, parts, floats;
+};
 
-// Pieces of each context: enough blocks to fill the GPU twice over, at least 128 keys a piece.  By sizes alone.
-static int kv4_splits(int n_seqs, int max_q_len, int table_width, int num_heads, int num_kv_heads, int block_size, int window, int sms) {
-    const long long most = (long long)table_width * block_size, keys = window > 0 && window + max_q_len < most ? window + max_q_len : most;
-    const long long blocks = (long long)n_seqs * num_kv_heads * kv4_row_tiles(max_q_len, num_heads / num_kv_heads);
-    const long long by_length = keys / 128, by_count = (2 * sms + blocks - 1) / blocks;
-    long long splits = by_length < by_count ? by_length : by_count;
-    return (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+static Kv4Plan kv4_plan(int n_seqs, int max_q_len, int table_width, int num_heads, int num_kv_heads, int block_size, int window, int sms) {
+    Kv4Plan plan;
+    const long long rows = (long long)max_q_len * (num_heads / num_kv_heads);
+    plan.tiles_of_8 = rows > 8 ? 2 : 1;
+    plan.chunk = block_size % 32 == 0 ? 32 : 16;
+    const int row_tiles = (int)((rows + 8 * plan.tiles_of_8 - 1) / (8 * plan.tiles_of_8));
+    const long long most = (long long)table_width * block_size, span = window > 0 && window + max_q_len - 1 < most ? window + max_q_len - 1 : most;
+    const long long chunks = span < most ? (span + plan.chunk - 2) / plan.chunk + 1 : most / plan.chunk;       // of an item
+    plan.items = (long long)n_seqs * num_kv_heads * row_tiles;
+    plan.chunks = plan.items * chunks;
+    const long long resident = (long long)sms * (plan.tiles_of_8 == 1 && FHD <= 128 ? 2 : 1);
+    constexpr int least = 1;                          // (at least 4: 1 x 300 positions 9.2 us against 7.2, 4 x 5 tokens over 4,000 19.0 against 17.5)
+    const long long wanted = (plan.chunks + least - 1) / least;
+    plan.blocks = (int)(wanted < resident ? wanted : resident);
+    const long long workers = (long long)plan.blocks * KV4_WARPS, run = plan.chunks / workers > least ? plan.chunks / workers : least;
+    plan.cut = {n_seqs, num_heads, num_kv_heads, window, least, (int)most, row_tiles};
+    plan.parts = chunks > 1 ? (chunks + run - 1) / run + 1 : 1;
+    plan.floats = plan.parts > 1 ? 2 * workers * 8 * plan.tiles_of_8 * (FPAD + 2) : 0;
+    return plan;
 }
 
-template <int NT>
-static int kv4_launch(const void* q, const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int* block_table,
-                      int table_width, const int* cu_q, const int* ctx_after, void* out, float* scratch, int n_seqs, int n_tokens, int num_heads,
-                      int num_kv_heads, int block_size, float scale, int window, int splits, int row_tiles, cudaStream_t stream) {
-    const size_t smem = (size_t)KV4_WARPS * 8 * NT * (FHD + 2) * sizeof(float);
-    if (int code = reserve_shared_once<kv4_attention_kernel<NT>>("skv_attention_kv4", smem)) return code;
-    float* partial_o = scratch;
-    float* partial_ml = scratch ? scratch + (size_t)n_tokens * num_heads * splits * FHD : nullptr;
-    if (int code = launch_pdl("skv_attention_kv4", kv4_attention_kernel<NT>, dim3(n_seqs, num_kv_heads * row_tiles, splits), dim3(KV4_WARPS * 32), smem,
-                              stream, (const __nv_bfloat16*)q, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale,
-                              (const uint8_t*)v_scale, block_table, table_width, cu_q, ctx_after, (__nv_bfloat16*)out, partial_o, partial_ml, num_heads,
-                              num_kv_heads, block_size, scale, window, splits, row_tiles))
+template <int NT, int CK>
+static int kv4_launch(const Kv4Plan& plan, const void* q, const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale,
+                      const int* block_table, int table_width, const int* cu_q, const int* ctx_after, void* out, float* scratch, int block_size,
+                      float scale, cudaStream_t stream) {
+    // a chunk's block is chunk / (block_size / CK): the upper half of a product, exact while chunks x chunks a block stay below 2^32
+    const uint32_t chunks_magic = block_size == CK ? 0u : (uint32_t)((0x100000000ull + block_size / CK - 1) / (block_size / CK));
+    if (int code = reserve_shared_once<kv4_attention_kernel<NT, CK>>("skv_attention_kv4", RING_OF<CK>)) return code;
+    const int workers = plan.blocks * KV4_WARPS;
+    float* partial_ml = plan.floats ? scratch + (size_t)2 * workers * 8 * NT * FPAD : nullptr;
+    if (int code = launch_pdl("skv_attention_kv4", kv4_attention_kernel<NT, CK>, dim3(plan.blocks), dim3(KV4_WARPS * 32), RING_OF<CK>, stream,
+                              (const __nv_bfloat16*)q, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
+                              block_table, table_width, cu_q, ctx_after, (__nv_bfloat16*)out, (float4*)scratch, (float2*)partial_ml, plan.cut, block_size,
+                              scale, chunks_magic, KV4_ONES))
         return code;
-    if (splits == 1) return 0;
-    return launch_pdl("skv_attention_kv4(combine)", kv4_combine_kernel, dim3(n_tokens * num_heads), dim3(KV4_COMBINE_THREADS), 0, stream,
-                      (const float*)partial_o, (const float*)partial_ml, cu_q, (__nv_bfloat16*)out, n_seqs, num_heads, splits);
+    if (plan.floats == 0) return 0;
+    const bool spread = plan.parts > 9 && plan.items < sm_count();
+    auto merge = spread ? kv4_merge_kernel<NT, CK, true> : kv4_merge_kernel<NT, CK, false>;
+    return launch_pdl("skv_attention_kv4(merge)", merge, dim3((unsigned)plan.items, spread ? OTILE4 * NT : 1), dim3(KV4_WARPS * 32), 0, stream,
+                      (const float4*)scratch, (const float4*)partial_ml, cu_q, ctx_after, (__nv_bfloat16*)out, plan.cut, workers);
 }
 
 }  // namespace skv
@@ -382,43 +678,44 @@ static int kv4_launch(const void* q, const void* k_codes, const void* v_codes, c
 using namespace skv;
 
 // Floats of scratch that a call of these sizes needs (0: none).
-SKV_EXPORT long long skv_attention_kv4_scratch(int n_seqs, int n_tokens, int max_q_len, int table_width, int num_heads, int num_kv_heads,
-                                               int block_size, int window) {
-    if (n_seqs <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads) return 0;
-    const int splits = kv4_splits(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window, sm_count());
-    return splits > 1 ? (long long)n_tokens * num_heads * splits * (FHD + 2) : 0;
+SKV_EXPORT long long skv_attention_kv4_scratch(int n_seqs, int max_q_len, int table_width, int num_heads, int num_kv_heads, int block_size,
+                                               int window) {
+    if (n_seqs <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || block_size <= 0) return 0;
+    return kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window, sm_count()).floats;
 }
 
-// Sequence s owns rows cu_q[s] .. cu_q[s+1]-1 of q and out ([tokens][heads][head_dim]); ctx_after[s] positions are cached, its own included.
+// Sequence s owns rows cu_q[s] .. cu_q[s+1]-1 of q and out ([tokens][heads][head_dim]), at most max_q_len; ctx_after[s] positions are cached, its own
+// included, at most table_width blocks of them.
 SKV_EXPORT int skv_attention_kv4(const void* q, const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale,
                                  const int* block_table, int table_width, const int* cu_q, const int* ctx_after, void* out, float* scratch,
-                                 long long scratch_floats, int n_seqs, int n_tokens, int max_q_len, int num_heads, int num_kv_heads,
-                                 int head_dim, int block_size, float scale, int window, cudaStream_t stream) {
-    if (n_seqs <= 0 || n_tokens <= 0 || max_q_len <= 0) return 0;
+                                 long long scratch_floats, int n_seqs, int max_q_len, int num_heads, int num_kv_heads, int head_dim,
+                                 int block_size, float scale, int window, cudaStream_t stream) {
+    if (n_seqs <= 0 || max_q_len <= 0 || table_width <= 0) return 0;
+    if (n_seqs > KV4_SEQS) return fail("skv_attention_kv4", "at most 1,024 sequences in a call");
     if (head_dim != FHD) return fail("skv_attention_kv4", "this library was built for another head size");
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
         return fail("skv_attention_kv4", "heads must be a positive multiple of kv heads");
     if (block_size <= 0 || block_size % 16 != 0) return fail("skv_attention_kv4", "block_size must be a positive multiple of 16");
     if (window < 0) return fail("skv_attention_kv4", "a window must not be negative");
-    if (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)out) & 15)
+    if ((unsigned long long)num_kv_heads * block_size * FHD > 0x80000000ull) return fail("skv_attention_kv4", "a cache block is too large (2 GB at most)");
+    if ((unsigned long long)table_width * (block_size / 16) * (block_size / 16) >= 0x100000000ull || (unsigned long long)table_width * block_size > 0x7fffffffull)
+        return fail("skv_attention_kv4", "the block table spans too many positions for blocks of this size");
+    if (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)out | (uintptr_t)scratch) & 15)
         return fail("skv_attention_kv4", "operands must be 16-byte aligned");
-    const int row_tiles = kv4_row_tiles(max_q_len, num_heads / num_kv_heads);
-    if ((long long)num_kv_heads * row_tiles > 65535) return fail("skv_attention_kv4", "too many rows in one step (kv heads x tiles of 16 rows: 65,535 at most)");
-    if ((long long)n_tokens * num_heads > 0x7fffffffLL) return fail("skv_attention_kv4", "too many rows in one step");
-    const int splits = kv4_splits(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window, sm_count());
-    if (splits > 1 && (!scratch || scratch_floats < (long long)n_tokens * num_heads * splits * (FHD + 2)))
-        return fail("skv_attention_kv4", "scratch is too small");
-    auto launch = max_q_len * (num_heads / num_kv_heads) > 8 ? kv4_launch<2> : kv4_launch<1>;
-    return launch(q, k_codes, v_codes, k_scale, v_scale, block_table, table_width, cu_q, ctx_after, out, scratch, n_seqs, n_tokens, num_heads,
-                  num_kv_heads, block_size, scale, window, splits, row_tiles, stream);
+    if ((long long)n_seqs * max_q_len * num_heads > 0x3fffffffLL) return fail("skv_attention_kv4", "too many rows in one step");
+    const Kv4Plan plan = kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window, sm_count());
+    if (plan.chunks > 0x7fffffffLL) return fail("skv_attention_kv4", "too many rows and positions in one step");
+    if (plan.floats && (!scratch || scratch_floats < plan.floats)) return fail("skv_attention_kv4", "scratch is too small");
+    auto launch = plan.tiles_of_8 == 2 ? (plan.chunk == 32 ? kv4_launch<2, 32> : kv4_launch<2, 16>) : plan.chunk == 32 ? kv4_launch<1, 32> : kv4_launch<1, 16>;
+    return launch(plan, q, k_codes, v_codes, k_scale, v_scale, block_table, table_width, cu_q, ctx_after, out, scratch, block_size, scale, stream);
 }
 
 #else
 
-SKV_EXPORT long long skv_attention_kv4_scratch(int, int, int, int, int, int, int, int) { return 0; }
+SKV_EXPORT long long skv_attention_kv4_scratch(int, int, int, int, int, int, int) { return 0; }
 
 SKV_EXPORT int skv_attention_kv4(const void*, const void*, const void*, const void*, const void*, const int*, int, const int*, const int*,
-                                 void*, float*, long long, int, int, int, int, int, int, int, float, int, cudaStream_t) {
+                                 void*, float*, long long, int, int, int, int, int, int, float, int, cudaStream_t) {
     return skv::fail("skv_attention_kv4", "a 4-bit cache is built for bfloat16");
 }
 

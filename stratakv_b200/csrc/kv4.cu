@@ -8,24 +8,95 @@
 
 namespace skv {
 
-// A thread has four neighbouring numbers of a head of the float32 row [q | k | v]; four lanes have a group of 16.  Queries and keys are
-// rotated (number i with number i + head_dim / 2; products and sum rounded one by one, so that a code never depends on how an
-// expression was compiled), queries rounded to bfloat16, keys and values to codes.
+// Queries and keys of the float32 rows [q | k | v] are rotated (number i with number i + head_dim / 2; products and sum rounded one by one, so that a
+// code never depends on how an expression was compiled), queries rounded to bfloat16, keys and values to codes.  Bound by the rows it
+// reads once there are enough of them.
 constexpr int APPEND_THREADS = 256;
 
-__global__ void __launch_bounds__(APPEND_THREADS)
+// Codes and scale byte of a group of 16 whose numbers four neighbouring lanes have, four each.
+__device__ __forceinline__ void kv4_store_group(const float (&v)[4], uint8_t* codes, uint8_t* scale, unsigned int mates) {
+    // magnitudes are ordered as their bits are, infinities and NaN above the rest
+    uint32_t bits = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits = max(bits, __float_as_uint(v[i]) & 0x7fffffffu);
+    bits = max(bits, __shfl_xor_sync(mates, bits, 1));
+    bits = max(bits, __shfl_xor_sync(mates, bits, 2));
+    const bool finite = bits < 0x7f800000u;
+    const uint32_t byte = finite ? kv4_scale_byte(__uint_as_float(bits)) : KV4_NOT_FINITE;
+    const float inverse = finite && byte ? __frcp_rn(kv4_scale(byte)) : 0.0f;
+    uint32_t packed = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) packed |= kv4_code(v[i], inverse) << (4 * i);
+    if (!finite) packed = 0x8888u;
+    *(unsigned short*)codes = (unsigned short)packed;
+    if ((threadIdx.x & 3) == 0) *scale = (uint8_t)byte;
+}
+__device__ __forceinline__ void kv4_store_query(const float (&v)[4], __nv_bfloat16* to) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+    *(uint2*)to = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+}
+__device__ __forceinline__ float turned_low(float x, float y, float c, float s) { return __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)); }
+__device__ __forceinline__ float turned_high(float x, float y, float c, float s) { return __fadd_rn(__fmul_rn(x, s), __fmul_rn(y, c)); }
+
+// Head sizes that are multiples of 32, whose halves are whole groups: a thread has four neighbouring numbers and the four half a head further.  (Three such
+// pairs a thread, 71 registers: 2,048 tokens of 32 + 2 x 8 heads of 128, read back, 30.7 us against 21.8.)
+__global__ void __launch_bounds__(APPEND_THREADS, 8)
 kv4_append_kernel(const float* __restrict__ qkv, const float* __restrict__ cos_sin, const int* __restrict__ positions,
                   const int* __restrict__ token_seq, const int* __restrict__ block_table, int table_width,
                   __nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ v_codes,
                   uint8_t* __restrict__ k_scale, uint8_t* __restrict__ v_scale, int num_heads, int num_kv_heads, int head_dim,
-                  int block_size, int write_kv) {
+                  int block_size, int write_kv, uint32_t quads_magic) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = blockIdx.x, half = head_dim >> 1, quads = half >> 2;
+    const int item = blockIdx.y * APPEND_THREADS + threadIdx.x;
+    const int head = (int)__umulhi((uint32_t)item, quads_magic), d = (item - head * quads) << 2;          // item / quads
+    if (head >= num_heads + (write_kv ? 2 * num_kv_heads : 0)) return;     // (whole groups: half a head is a multiple of four quads)
+    const float* row = qkv + (size_t)t * (num_heads + 2 * num_kv_heads) * head_dim + (size_t)head * head_dim + d;
+    const float4 x = *(const float4*)row, y = *(const float4*)(row + half);
+    const int pos = positions[t];
+    float low[4] = {x.x, x.y, x.z, x.w}, high[4] = {y.x, y.y, y.z, y.w};
+    if (cos_sin && head < num_heads + num_kv_heads) {
+        const float4* at = (const float4*)(cos_sin + (size_t)pos * head_dim + 2 * d);       // (cos, sin) of four pairs
+        const float4 a = at[0], b = at[1];
+        const float c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float l = low[i], h = high[i];
+            low[i] = turned_low(l, h, c[i], s[i]);
+            high[i] = turned_high(l, h, c[i], s[i]);
+        }
+    }
+    if (head < num_heads) {
+        __nv_bfloat16* to = q_out + ((size_t)t * num_heads + head) * head_dim + d;
+        kv4_store_query(low, to);
+        kv4_store_query(high, to + half);
+        return;
+    }
+    const bool value = head >= num_heads + num_kv_heads;
+    const int kv_head = head - num_heads - (value ? num_kv_heads : 0);
+    const int block = block_table[(size_t)token_seq[t] * table_width + pos / block_size];
+    const size_t at = ((size_t)block * num_kv_heads + kv_head) * block_size + pos % block_size;
+    uint8_t* codes = (value ? v_codes : k_codes) + at * half + (d >> 1);
+    uint8_t* scale = (value ? v_scale : k_scale) + at * (head_dim >> 4) + (d >> 4);
+    const unsigned int mates = 0xFu << (threadIdx.x & 28);
+    kv4_store_group(low, codes, scale, mates);
+    kv4_store_group(high, codes + (half >> 1), scale + (half >> 4), mates);
+}
+
+// Other head sizes: a thread has four neighbouring numbers, and reads those half a head away for its rotation.
+__global__ void __launch_bounds__(APPEND_THREADS)
+kv4_append_odd_kernel(const float* __restrict__ qkv, const float* __restrict__ cos_sin, const int* __restrict__ positions,
+                      const int* __restrict__ token_seq, const int* __restrict__ block_table, int table_width,
+                      __nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_codes, uint8_t* __restrict__ v_codes,
+                      uint8_t* __restrict__ k_scale, uint8_t* __restrict__ v_scale, int num_heads, int num_kv_heads, int head_dim,
+                      int block_size, int write_kv, uint32_t quads_magic) {
     pdl_launch_dependents();
     pdl_wait();
     const int t = blockIdx.x, quads = head_dim >> 2, half = head_dim >> 1;
     const int item = blockIdx.y * APPEND_THREADS + threadIdx.x;
-    const int head = item / quads, d = (item - head * quads) << 2;
-    const int all_heads = num_heads + (write_kv ? 2 * num_kv_heads : 0);
-    if (head >= all_heads) return;                     // (whole groups: a head is a multiple of four quads)
+    const int head = (int)__umulhi((uint32_t)item, quads_magic), d = (item - head * quads) << 2;
+    if (head >= num_heads + (write_kv ? 2 * num_kv_heads : 0)) return;     // (whole groups: a head is a multiple of four quads)
     const int pos = positions[t];
     const float* x = qkv + (size_t)t * (num_heads + 2 * num_kv_heads) * head_dim + (size_t)head * head_dim;
     const float4 own = *(const float4*)(x + d);
@@ -34,40 +105,27 @@ kv4_append_kernel(const float* __restrict__ qkv, const float* __restrict__ cos_s
         const bool low = d < half;
         const float4 other = *(const float4*)(x + (low ? d + half : d - half));
         const float4* at = (const float4*)(cos_sin + (size_t)pos * head_dim + 2 * (low ? d : d - half));
-        const float4 a = at[0], b = at[1];             // (cos, sin) of four pairs
+        const float4 a = at[0], b = at[1];
         const float w[4] = {other.x, other.y, other.z, other.w}, c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i] = low ? __fsub_rn(__fmul_rn(v[i], c[i]), __fmul_rn(w[i], s[i])) : __fadd_rn(__fmul_rn(w[i], s[i]), __fmul_rn(v[i], c[i]));
+        for (int i = 0; i < 4; ++i) v[i] = low ? turned_low(v[i], w[i], c[i], s[i]) : turned_high(w[i], v[i], c[i], s[i]);
     }
     if (head < num_heads) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-        *(uint2*)(q_out + ((size_t)t * num_heads + head) * head_dim + d) = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+        kv4_store_query(v, q_out + ((size_t)t * num_heads + head) * head_dim + d);
         return;
     }
     const bool value = head >= num_heads + num_kv_heads;
     const int kv_head = head - num_heads - (value ? num_kv_heads : 0);
     const int block = block_table[(size_t)token_seq[t] * table_width + pos / block_size];
     const size_t row = ((size_t)block * num_kv_heads + kv_head) * block_size + pos % block_size;
-    const unsigned int mates = 0xFu << (threadIdx.x & 28);
-    float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    bool finite = isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3]);
-    most = fmaxf(most, __shfl_xor_sync(mates, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(mates, most, 2));
-    finite = __all_sync(mates, finite);
-    const uint32_t byte = finite ? kv4_scale_byte(most) : KV4_NOT_FINITE;
-    const float inverse = finite && byte ? __frcp_rn(kv4_scale(byte)) : 0.0f;
-    uint32_t codes = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) codes |= kv4_code(finite ? v[i] : 0.0f, inverse) << (4 * i);
-    *(unsigned short*)((value ? v_codes : k_codes) + row * (head_dim >> 1) + (d >> 1)) = (unsigned short)codes;
-    if ((threadIdx.x & 3) == 0) (value ? v_scale : k_scale)[row * (head_dim >> 4) + (d >> 4)] = (uint8_t)byte;
+    kv4_store_group(v, (value ? v_codes : k_codes) + row * half + (d >> 1), (value ? v_scale : k_scale) + row * (head_dim >> 4) + (d >> 4),
+                    0xFu << (threadIdx.x & 28));
 }
 
 // Blocks of the cache as the bfloat16 numbers they stand for.  Block i of sequence s is its logical block first + i, where `first` holds
 // the oldest of the last `keep` positions (0: all of them); rows behind the sequence's end are zero.  out_table[s][b] is where logical
 // block b went (0 for those before the first, which nobody may read).
-constexpr int UNPACK_THREADS = 256;
+constexpr int UNPACK_THREADS = 256, UNPACK_ITEMS = 4;          // words of eight codes that a thread has on their way at once
 
 __global__ void __launch_bounds__(UNPACK_THREADS)
 kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ k_scale,
@@ -79,7 +137,7 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
     const int seq = blockIdx.x / out_width, i = blockIdx.x - seq * out_width, kv_head = blockIdx.y;
     const int ctx = ctx_after[seq];
     const int first = keep > 0 ? max(0, ctx - keep) / block_size : 0, logical = first + i;
-    if (kv_head == 0) {
+    if (kv_head == 0 && blockIdx.z == 0) {
         if (threadIdx.x == 0 && logical < table_width) out_table[(size_t)seq * table_width + logical] = blockIdx.x;
         if (i == 0)
             for (int b = threadIdx.x; b < table_width; b += UNPACK_THREADS)
@@ -89,24 +147,36 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
     const int block = logical < table_width && rows > 0 ? block_table[(size_t)seq * table_width + logical] : 0;
     const size_t from = ((size_t)block * num_kv_heads + kv_head) * block_size;
     const size_t to = ((size_t)blockIdx.x * num_kv_heads + kv_head) * block_size;
-    const int words = head_dim >> 3;                                      // of eight numbers
-    for (int idx = threadIdx.x; idx < 2 * block_size * words; idx += UNPACK_THREADS) {
-        const bool value = idx >= block_size * words;
-        const int at = idx - (value ? block_size * words : 0), row = at / words, w = at - row * words;
-        uint4 out = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) {
-            const uint32_t word = *(const uint32_t*)((value ? v_codes : k_codes) + (from + row) * (head_dim >> 1) + 4 * w);
-            const float s = kv4_scale((value ? v_scale : k_scale)[(from + row) * (head_dim >> 4) + (w >> 1)]);
+    const int words = head_dim >> 3, of_one = block_size * words;          // words of eight numbers
+    constexpr int ITEMS = UNPACK_ITEMS;
+    for (int first_item = threadIdx.x + blockIdx.z * ITEMS * UNPACK_THREADS; first_item < 2 * of_one;
+         first_item += gridDim.z * ITEMS * UNPACK_THREADS) {
+        uint32_t word[ITEMS], byte[ITEMS];
+        size_t target[ITEMS];
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u) {
+            const int idx = first_item + u * UNPACK_THREADS;
+            const bool value = idx >= of_one;
+            const int at = idx - (value ? of_one : 0), row = at / words, w = at - row * words;
+            const bool live = idx < 2 * of_one && row < rows;
+            word[u] = live ? *(const uint32_t*)((value ? v_codes : k_codes) + (from + row) * (head_dim >> 1) + 4 * w) : 0u;
+            byte[u] = live ? (value ? v_scale : k_scale)[(from + row) * (head_dim >> 4) + (w >> 1)] : 0u;
+            target[u] = (to + row) * head_dim + 8 * w;
+        }
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u) {
+            const int idx = first_item + u * UNPACK_THREADS;
+            if (idx >= 2 * of_one) break;
+            const float s = kv4_scale(byte[u]);                            // (0 behind the sequence's end, and so is all that it scales)
             uint32_t packed[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 pair = __floats2bfloat162_rn((float)((int)(word >> (8 * e) & 15u) - 8) * s,
-                                                                  (float)((int)(word >> (8 * e + 4) & 15u) - 8) * s);
-                packed[e] = *(const uint32_t*)&pair;
+                const __nv_bfloat162 pair = __floats2bfloat162_rn((float)((int)(word[u] >> (8 * e) & 15u) - 8) * s,
+                                                                  (float)((int)(word[u] >> (8 * e + 4) & 15u) - 8) * s);
+                packed[e] = byte[u] ? *(const uint32_t*)&pair : 0u;        // (no negative zero)
             }
-            out = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+            *(uint4*)((idx >= of_one ? v_out : k_out) + target[u]) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
         }
-        *(uint4*)((value ? v_out : k_out) + (to + row) * head_dim + 8 * w) = out;
     }
 }
 
@@ -125,12 +195,18 @@ SKV_EXPORT int skv_append_kv4(const float* qkv, const float* cos_sin, const int*
         return fail("skv_append_kv4", "heads must be a positive multiple of kv heads");
     if (block_size <= 0 || block_size % 16 != 0) return fail("skv_append_kv4", "block_size must be a positive multiple of 16");
     if (((uintptr_t)qkv | (uintptr_t)cos_sin | (uintptr_t)q_out) & 15) return fail("skv_append_kv4", "operands must be 16-byte aligned");
-    const long long items = (long long)(num_heads + (write_kv ? 2 * num_kv_heads : 0)) * (head_dim / 4);
+    // twice four numbers a thread, or four
+    const bool paired = head_dim % 32 == 0;
+    const long long items = (long long)(num_heads + (write_kv ? 2 * num_kv_heads : 0)) * (head_dim / (paired ? 8 : 4));
     const long long pieces = (items + APPEND_THREADS - 1) / APPEND_THREADS;
     if (pieces > 65535) return fail("skv_append_kv4", "a row of queries, keys and values is too long");
-    return launch_pdl("skv_append_kv4", kv4_append_kernel, dim3(n_tokens, (unsigned)pieces), dim3(APPEND_THREADS), 0, stream, qkv, cos_sin,
-                      positions, token_seq, block_table, table_width, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)v_codes,
-                      (uint8_t*)k_scale, (uint8_t*)v_scale, num_heads, num_kv_heads, head_dim, block_size, write_kv);
+    // item / quads as the upper half of a product: exact while items x quads stay below 2^32
+    const uint32_t quads = head_dim / (paired ? 8 : 4), quads_magic = (uint32_t)((0x100000000ull + quads - 1) / quads);
+    if ((items + APPEND_THREADS) * quads >= 0x100000000ll) return fail("skv_append_kv4", "a row of queries, keys and values is too long");
+    auto kernel = paired ? kv4_append_kernel : kv4_append_odd_kernel;
+    return launch_pdl("skv_append_kv4", kernel, dim3(n_tokens, (unsigned)pieces), dim3(APPEND_THREADS), 0, stream, qkv, cos_sin, positions, token_seq,
+                      block_table, table_width, (__nv_bfloat16*)q_out, (uint8_t*)k_codes, (uint8_t*)v_codes, (uint8_t*)k_scale, (uint8_t*)v_scale,
+                      num_heads, num_kv_heads, head_dim, block_size, write_kv, quads_magic);
 }
 
 SKV_EXPORT int skv_unpack_kv4(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int* block_table,
@@ -144,7 +220,10 @@ SKV_EXPORT int skv_unpack_kv4(const void* k_codes, const void* v_codes, const vo
     if ((long long)n_seqs * out_width > 0x7fffffffLL) return fail("skv_unpack_kv4", "too many blocks");
     if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
         return fail("skv_unpack_kv4", "operands must be 16-byte aligned");
-    return launch_pdl("skv_unpack_kv4", kv4_unpack_kernel, dim3((unsigned)(n_seqs * out_width), (unsigned)num_kv_heads), dim3(UNPACK_THREADS), 0,
+    const long long items = 2ll * block_size * (head_dim / 8);
+    if (items > 0x40000000ll) return fail("skv_unpack_kv4", "a cache block is too large");
+    const long long wanted = (items + UNPACK_ITEMS * UNPACK_THREADS - 1) / (UNPACK_ITEMS * UNPACK_THREADS), parts = wanted < 64 ? wanted : 64;
+    return launch_pdl("skv_unpack_kv4", kv4_unpack_kernel, dim3((unsigned)(n_seqs * out_width), (unsigned)num_kv_heads, (unsigned)parts), dim3(UNPACK_THREADS), 0,
                       stream, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table,
                       table_width, ctx_after, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_table, out_width, num_kv_heads, head_dim,
                       block_size, keep);

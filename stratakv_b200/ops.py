@@ -34,6 +34,7 @@ LOW_RANK_PLAIN, LOW_RANK_LOG_SIGMOID, LOW_RANK_SOFTPLUS = 0, 1, 2
 STEP_CHANNEL, STEP_DELTA, STEP_EXP = 0, 1, 2
 # query rows a key head (heads of a group x new tokens of a sequence) up to which ``attention_kv4`` reads the 4-bit cache itself
 KV4_FEW_ROWS = 64
+KV4_SEQS = 1024            # sequences that one launch of it takes (csrc/attention_kv4.cu)
 MAX_STREAMS = 8            # copies of the residual stream that ``stream_mix`` takes (csrc/stream_mix.cu)
 
 
@@ -64,7 +65,8 @@ _SCOPED_STREAM = None
 def _stream():
     if _SCOPED_STREAM is not None:
         return _SCOPED_STREAM
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the stream's address itself: making a torch.cuda.Stream of it costs the host 3.7 us a call)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 class stream_scope:
@@ -1450,39 +1452,63 @@ class Kernels:
             *self._state_args(step_meta, state, state_offset), _stream()), "matrix_step")
 
     # ---- a cache held in 4 bits (csrc/kv4.cuh) --------------------------------------------------------------------
+    # (These calls check their tensors in one go and hand plain addresses to prototyped functions: a step has two of them a layer, and
+    # with a check and a pointer object per tensor the host took 21 us for the one and 17 for the other.)
+    _kv4_prototyped = False
+
     def has_kv4(self) -> bool:
         return bool(self.lib.skv_has_kv4())
 
-    def _kv4_cache(self, k_codes, v_codes, k_scale, v_scale, num_kv_heads: int, head_dim: int, block_size: int, name: str) -> None:
-        for what, tensor, width in (("k_codes", k_codes, head_dim // 2), ("v_codes", v_codes, head_dim // 2),
-                                    ("k_scale", k_scale, head_dim // 16), ("v_scale", v_scale, head_dim // 16)):
-            self._want(tensor, torch.uint8, what)
-            if tuple(tensor.shape[1:]) != (num_kv_heads, block_size, width) or tensor.shape[0] != k_codes.shape[0]:
-                raise KernelError(f"{name}: {what} must be [blocks, kv_heads, block_size, {width}]")
+    def _kv4_prototypes(self) -> None:
+        p, i = ctypes.c_void_p, ctypes.c_int
+        self.lib.skv_append_kv4.argtypes = [p] * 5 + [i] + [p] * 5 + [i] * 6 + [p]
+        self.lib.skv_unpack_kv4.argtypes = [p] * 5 + [i] + [p] * 4 + [i] * 6 + [p]
+        self.lib.skv_attention_kv4.argtypes = [p] * 6 + [i] + [p] * 4 + [ctypes.c_longlong] + [i] * 6 + [ctypes.c_float, i, p]
+        self.lib.skv_attention_kv4_scratch.argtypes = [i] * 7
+        self.lib.skv_attention_kv4_scratch.restype = ctypes.c_longlong
+        self._kv4_plans = {}
+        self._kv4_prototyped = True
+
+    def _want_all(self, call: str, *wanted) -> None:
+        """``wanted``: (tensor, dtype, name) each; all of them contiguous, and on the current device."""
+        if not self._kv4_prototyped:
+            self._kv4_prototypes()
+        device = torch.cuda.current_device() if wanted[0][0].is_cuda else -1
+        for tensor, dtype, name in wanted:
+            if tensor.dtype is not dtype or tensor.get_device() != device or device < 0 or not tensor.is_contiguous():
+                self._want(tensor, dtype, name)
+                raise KernelError(f"{call}: {name} is on another device than the current one")
+
+    def _kv4_cache(self, call: str, k_codes, v_codes, k_scale, v_scale, num_kv_heads: int, head_dim: int, block_size: int) -> None:
+        codes = (k_codes.shape[0], num_kv_heads, block_size, head_dim // 2)
+        scales = (k_codes.shape[0], num_kv_heads, block_size, head_dim // 16)
+        if k_codes.shape != codes or v_codes.shape != codes or k_scale.shape != scales or v_scale.shape != scales:
+            raise KernelError(f"{call}: k_codes and v_codes must be [blocks, kv_heads, block_size, {head_dim // 2}], "
+                              f"k_scale and v_scale [blocks, kv_heads, block_size, {head_dim // 16}]")
 
     def append_kv4(self, qkv, cos_sin, positions, token_seq, block_table, q_out, k_codes, v_codes, k_scale, v_scale, num_heads: int,
                    num_kv_heads: int, head_dim: int, block_size: int, write_kv: bool = True):
         """``rope_kv_write`` into a cache held in 4 bits (bfloat16 build, head sizes that are multiples of 16): codes uint8
         ``[blocks, kv_heads, block_size, head_dim / 2]``, scales uint8 ``[..., head_dim / 16]``.  A token's position must not come twice
         in a call.  Numbers beyond 6,272 saturate; a group of 16 with an infinity or a NaN reads as NaN."""
-        self._want(qkv, torch.float32, "qkv"); self._want(q_out, self.dtype, "q_out")
-        self._want(positions, torch.int32, "positions"); self._want(token_seq, torch.int32, "token_seq")
-        self._want(block_table, torch.int32, "block_table")
+        u8, i32 = torch.uint8, torch.int32
+        self._want_all("append_kv4", (qkv, torch.float32, "qkv"), (q_out, self.dtype, "q_out"), (positions, i32, "positions"),
+                       (token_seq, i32, "token_seq"), (block_table, i32, "block_table"), (k_codes, u8, "k_codes"), (v_codes, u8, "v_codes"),
+                       (k_scale, u8, "k_scale"), (v_scale, u8, "v_scale"))
         if cos_sin is not None:
-            self._want(cos_sin, torch.float32, "cos_sin")
+            self._want_all("append_kv4", (cos_sin, torch.float32, "cos_sin"))
             if cos_sin.numel() % head_dim:
                 raise KernelError("append_kv4: a row of cos_sin must hold a pair for every two numbers of a head")
+        self._kv4_cache("append_kv4", k_codes, v_codes, k_scale, v_scale, num_kv_heads, head_dim, block_size)
         n = qkv.shape[0]
-        if write_kv:
-            self._kv4_cache(k_codes, v_codes, k_scale, v_scale, num_kv_heads, head_dim, block_size, "append_kv4")
         if qkv.dim() != 2 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
             raise KernelError("append_kv4: qkv width does not match the head counts")
-        if tuple(q_out.shape) != (n, num_heads * head_dim) or positions.numel() != n or token_seq.numel() != n or block_table.dim() != 2:
+        if q_out.shape != (n, num_heads * head_dim) or positions.numel() != n or token_seq.numel() != n or block_table.dim() != 2:
             raise KernelError("append_kv4: one query row, one position and one sequence index per token is needed")
         self._check(self.lib.skv_append_kv4(
-            _ptr(qkv), _ptr(cos_sin), _ptr(positions), _ptr(token_seq), _ptr(block_table), block_table.shape[1], _ptr(q_out), _ptr(k_codes),
-            _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), n, num_heads, num_kv_heads, head_dim, block_size, int(bool(write_kv)),
-            _stream()), "append_kv4")
+            qkv.data_ptr(), None if cos_sin is None else cos_sin.data_ptr(), positions.data_ptr(), token_seq.data_ptr(), block_table.data_ptr(),
+            block_table.shape[1], q_out.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, num_heads,
+            num_kv_heads, head_dim, block_size, 1 if write_kv else 0, _stream()), "append_kv4")
 
     def unpack_kv4(self, k_codes, v_codes, k_scale, v_scale, block_table, ctx_after, k_out, v_out, out_table, num_kv_heads: int,
                    head_dim: int, block_size: int, keep: int = 0):
@@ -1490,78 +1516,96 @@ class Kernels:
         ``[sequences * width, kv_heads, block_size, head_dim]`` get ``width`` blocks of each, from the one that holds the oldest of its last
         ``keep`` positions on (0: from its first block on); rows behind a sequence's end become zero.  ``out_table`` (int32, as
         ``block_table``) says where each logical block went, for attention over ``k_out`` and ``v_out``."""
-        self._kv4_cache(k_codes, v_codes, k_scale, v_scale, num_kv_heads, head_dim, block_size, "unpack_kv4")
-        self._want(block_table, torch.int32, "block_table"); self._want(ctx_after, torch.int32, "ctx_after")
-        self._want(k_out, self.dtype, "k_out"); self._want(v_out, self.dtype, "v_out"); self._want(out_table, torch.int32, "out_table")
+        u8, i32 = torch.uint8, torch.int32
+        self._want_all("unpack_kv4", (k_codes, u8, "k_codes"), (v_codes, u8, "v_codes"), (k_scale, u8, "k_scale"), (v_scale, u8, "v_scale"),
+                       (block_table, i32, "block_table"), (ctx_after, i32, "ctx_after"), (k_out, self.dtype, "k_out"),
+                       (v_out, self.dtype, "v_out"), (out_table, i32, "out_table"))
+        self._kv4_cache("unpack_kv4", k_codes, v_codes, k_scale, v_scale, num_kv_heads, head_dim, block_size)
         n_seqs = ctx_after.numel()
         if block_table.dim() != 2 or block_table.shape[0] != n_seqs or out_table.shape != block_table.shape:
             raise KernelError("unpack_kv4: one length and one row of either table per sequence is needed")
-        if (n_seqs == 0 or k_out.shape[0] % n_seqs or tuple(k_out.shape[1:]) != (num_kv_heads, block_size, head_dim)
+        if (n_seqs == 0 or k_out.shape[0] % n_seqs or k_out.shape != (k_out.shape[0], num_kv_heads, block_size, head_dim)
                 or k_out.shape != v_out.shape):
             raise KernelError("unpack_kv4: the results must be [sequences * width, kv_heads, block_size, head_dim]")
         if keep < 0:
             raise KernelError("unpack_kv4: the positions to keep must not be negative")
         self._check(self.lib.skv_unpack_kv4(
-            _ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), _ptr(block_table), block_table.shape[1], _ptr(ctx_after),
-            _ptr(k_out), _ptr(v_out), _ptr(out_table), n_seqs, k_out.shape[0] // n_seqs, num_kv_heads, head_dim, block_size, int(keep),
-            _stream()), "unpack_kv4")
+            k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+            ctx_after.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), out_table.data_ptr(), n_seqs, k_out.shape[0] // n_seqs, num_kv_heads,
+            head_dim, block_size, int(keep), _stream()), "unpack_kv4")
 
-    def _kv4_unpacked_width(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int,
-                            block_size: int, window: int) -> int:
-        """Blocks of each sequence that a step reads through ``unpack_kv4``; 0 where it reads the 4-bit cache itself."""
-        if max_q_len * (num_heads // num_kv_heads) <= KV4_FEW_ROWS or block_size & (block_size - 1):
-            return 0
-        if not (self.has_attention_prefill_tc() and n_seqs * -(-max_q_len // 128) <= 65535):
-            return 0
-        if window <= 0:
-            return table_width
-        return min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
+    def _kv4_plan(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                  window: int) -> Tuple[int, int]:
+        """How ``attention_kv4`` serves a step of these sizes: (blocks of each sequence that it reads through ``unpack_kv4``, 0
+        where it reads the 4-bit cache itself; bytes of scratch)."""
+        if not self._kv4_prototyped:
+            self._kv4_prototypes()
+        key = (n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
+        plan = self._kv4_plans.get(key)
+        if plan is not None:
+            return plan
+        width = 0
+        if (max_q_len * (num_heads // max(1, num_kv_heads)) > KV4_FEW_ROWS and block_size & (block_size - 1) == 0 and block_size >= 16
+                and self.has_attention_prefill_tc() and head_dim == self.head_dim and n_seqs * -(-max_q_len // 128) <= 65535):
+            width = table_width if window <= 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
+        if width:
+            wanted = 4 * n_seqs * width * num_kv_heads * block_size * head_dim + 4 * n_seqs * table_width
+        else:
+            wanted = 4 * self.lib.skv_attention_kv4_scratch(min(n_seqs, KV4_SEQS), max_q_len, table_width, num_heads, num_kv_heads,
+                                                            block_size, window)
+        if len(self._kv4_plans) > 4096:
+            self._kv4_plans.clear()
+        self._kv4_plans[key] = (width, wanted)
+        return width, wanted
 
     def attention_kv4_scratch(self, n_seqs: int, n_tokens: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int,
                               head_dim: int, block_size: int, window: int = 0) -> int:
         """Bytes of scratch that ``attention_kv4`` needs for a step of these sizes."""
-        width = self._kv4_unpacked_width(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
-        if width:
-            return 4 * n_seqs * width * num_kv_heads * block_size * head_dim + 4 * n_seqs * table_width
-        self.lib.skv_attention_kv4_scratch.restype = ctypes.c_longlong
-        return 4 * self.lib.skv_attention_kv4_scratch(n_seqs, n_tokens, max_q_len, table_width, num_heads, num_kv_heads, block_size, window)
+        return self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)[1]
 
     def attention_kv4(self, q, k_codes, v_codes, k_scale, v_scale, block_table, cu_q, ctx_after, out, max_q_len: int, num_heads: int,
                       num_kv_heads: int, head_dim: int, block_size: int, scale: float, window: int = 0, scratch=None, flag=None):
         """Causal attention over a cache held in 4 bits (bfloat16 build): sequence ``s`` owns rows ``cu_q[s]..cu_q[s+1]-1`` of
         ``q``/``out`` (at most ``max_q_len``), ``ctx_after[s]`` positions are cached, this step's included.  One or a few new tokens a sequence
         read the cache as it lies; many read the bfloat16 numbers it stands for (``unpack_kv4``, then
-        ``attention_prefill_tc``).  ``scratch``: uint8, at least ``attention_kv4_scratch`` bytes."""
-        self._want(q, self.dtype, "q"); self._want(out, self.dtype, "out")
-        self._kv4_cache(k_codes, v_codes, k_scale, v_scale, num_kv_heads, head_dim, block_size, "attention_kv4")
-        self._want(block_table, torch.int32, "block_table"); self._want(cu_q, torch.int32, "cu_q")
-        self._want(ctx_after, torch.int32, "ctx_after")
-        n_seqs, n = ctx_after.numel(), q.shape[0]
-        if cu_q.numel() != n_seqs + 1 or block_table.dim() != 2 or block_table.shape[0] != n_seqs:
+        ``attention_prefill_tc``).  ``scratch``: uint8, at least ``attention_kv4_scratch`` bytes; two steps that may run at once need one each.
+        A step's sums are cut by all its sequences' lengths, so that a sequence's result may differ in their order between batches."""
+        u8, i32 = torch.uint8, torch.int32
+        self._want_all("attention_kv4", (q, self.dtype, "q"), (out, self.dtype, "out"), (k_codes, u8, "k_codes"), (v_codes, u8, "v_codes"),
+                       (k_scale, u8, "k_scale"), (v_scale, u8, "v_scale"), (block_table, i32, "block_table"), (cu_q, i32, "cu_q"),
+                       (ctx_after, i32, "ctx_after"))
+        self._kv4_cache("attention_kv4", k_codes, v_codes, k_scale, v_scale, num_kv_heads, head_dim, block_size)
+        n_seqs, n, table_width = ctx_after.numel(), q.shape[0], block_table.shape[-1]
+        if cu_q.numel() != n_seqs + 1 or block_table.shape != (n_seqs, table_width):
             raise KernelError("attention_kv4: one length, one offset pair and one table row per sequence is needed")
-        if tuple(q.shape) != (n, num_heads * head_dim) or out.shape != q.shape or max_q_len < 1:
+        if q.shape != (n, num_heads * head_dim) or out.shape != q.shape or max_q_len < 1:
             raise KernelError("attention_kv4: q and out must be [tokens, heads * head_dim]")
-        table_width = block_table.shape[1]
-        wanted = self.attention_kv4_scratch(n_seqs, n, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
+        width, wanted = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
         if wanted:
-            self._want(scratch, torch.uint8, "scratch")
-            if scratch.numel() < wanted:
-                raise KernelError(f"attention_kv4: {wanted} bytes of scratch are needed, not {scratch.numel()}")
-        width = self._kv4_unpacked_width(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
+            if scratch is None or scratch.numel() < wanted:
+                raise KernelError(f"attention_kv4: {wanted} bytes of scratch are needed, not {0 if scratch is None else scratch.numel()}")
+            self._want_all("attention_kv4", (scratch, u8, "scratch"))
         if width:
-            size = 2 * n_seqs * width * num_kv_heads * block_size * head_dim
-            shape = (n_seqs * width, num_kv_heads, block_size, head_dim)
-            keys, values = (scratch[at:at + size].view(self.dtype).view(shape) for at in (0, size))
-            table = scratch[2 * size:2 * size + 4 * n_seqs * table_width].view(torch.int32).view(n_seqs, table_width)
-            self.unpack_kv4(k_codes, v_codes, k_scale, v_scale, block_table, ctx_after, keys, values, table, num_kv_heads, head_dim,
-                            block_size, window + max_q_len - 1 if window > 0 else 0)
-            self.attention_prefill_tc(q, keys, values, table, cu_q, ctx_after, out, max_q_len, num_heads, num_kv_heads, head_dim,
-                                      block_size, scale, window, flag)
+            # keys, values and their block table lie in the scratch one behind the other
+            blocks, keys = n_seqs * width, scratch.data_ptr()
+            values = keys + 2 * blocks * num_kv_heads * block_size * head_dim
+            table = values + 2 * blocks * num_kv_heads * block_size * head_dim
+            self._check(self.lib.skv_unpack_kv4(
+                k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), table_width,
+                ctx_after.data_ptr(), keys, values, table, n_seqs, width, num_kv_heads, head_dim, block_size,
+                window + max_q_len - 1 if window > 0 else 0, _stream()), "unpack_kv4")
+            pointer, zero = ctypes.c_void_p, ctypes.c_float(0.0)
+            self._check(self.lib.skv_attention_prefill_tc_extras(
+                _ptr(q), pointer(keys), pointer(values), blocks, pointer(table), table_width, _ptr(cu_q), _ptr(ctx_after), _ptr(out), n_seqs, n,
+                max_q_len, num_heads, num_kv_heads, head_dim, block_size, ctypes.c_float(scale), window, _NULL, 0, _NULL, 0, zero, 0, _NULL,
+                _ptr(flag if flag is not None else self.error_flag), _stream()), "attention_prefill_tc")
             return
-        self._check(self.lib.skv_attention_kv4(
-            _ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), _ptr(block_table), table_width, _ptr(cu_q),
-            _ptr(ctx_after), _ptr(out), _ptr(scratch) if wanted else _NULL, ctypes.c_longlong(wanted // 4), n_seqs, n, max_q_len, num_heads,
-            num_kv_heads, head_dim, block_size, ctypes.c_float(scale), window, _stream()), "attention_kv4")
+        for at in range(0, n_seqs, KV4_SEQS):                  # (int32 tensors: four bytes an entry)
+            self._check(self.lib.skv_attention_kv4(
+                q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                block_table.data_ptr() + 4 * at * table_width, table_width, cu_q.data_ptr() + 4 * at, ctx_after.data_ptr() + 4 * at,
+                out.data_ptr(), scratch.data_ptr() if wanted else None, wanted // 4, min(n_seqs - at, KV4_SEQS), max_q_len, num_heads,
+                num_kv_heads, head_dim, block_size, scale, window, _stream()), "attention_kv4")
 
     def softcap_inplace(self, x, cap: float):
         """``x = cap * tanh(x / cap)`` (float32)."""

@@ -134,14 +134,15 @@ def test_the_libraries_refuse_bad_sizes():
         code, message = unpack(**changes)
         assert code != 0 and match in message, (changes, message)
 
-    def attend(seqs=1, tokens=1, most=1, heads=4, kv=2, dim=64, block=16, window=0, q=null, width=1, floats=0, scratch=null):
-        code = lib.skv_attention_kv4(q, null, null, null, null, null, i(width), null, null, null, scratch, ctypes.c_longlong(floats), i(seqs), i(tokens), i(most),
+    def attend(seqs=1, most=1, heads=4, kv=2, dim=64, block=16, window=0, q=null, width=1, floats=0, scratch=null):
+        code = lib.skv_attention_kv4(q, null, null, null, null, null, i(width), null, null, null, scratch, ctypes.c_longlong(floats), i(seqs), i(most),
                                      i(heads), i(kv), i(dim), i(block), ctypes.c_float(1.0), i(window), null)
         return code, lib.skv_last_error().decode()
 
-    assert attend(seqs=0)[0] == 0 and attend(tokens=0)[0] == 0 and attend(most=0)[0] == 0
+    assert attend(seqs=0)[0] == 0 and attend(width=0)[0] == 0 and attend(most=0)[0] == 0
     for match, changes in (("another head size", dict(dim=128)), ("multiple of kv heads", dict(heads=3)), ("block_size", dict(block=8)),
-                           ("must not be negative", dict(window=-3)), ("aligned", dict(q=odd)), ("too many rows", dict(heads=4, kv=4, most=2 ** 20))):
+                           ("must not be negative", dict(window=-3)), ("aligned", dict(q=odd)), ("too many rows", dict(heads=64, kv=64, most=2 ** 25)),
+                           ("too many positions", dict(width=2 ** 30)), ("too large", dict(kv=4, block=2 ** 27)), ("aligned", dict(scratch=odd))):
         code, message = attend(**changes)
         assert code != 0 and match in message, (changes, message)
 
@@ -152,6 +153,6 @@ def test_float32_libraries_have_none():
     assert lib.skv_has_kv4() == 0 and library("bfloat16", 64).skv_has_kv4() == 1
     assert lib.skv_append_kv4(null, null, null, null, null, i(1), null, null, null, null, null, i(1), i(1), i(1), i(64), i(16), i(1), null) != 0
     assert b"bfloat16" in lib.skv_last_error()
-    assert lib.skv_attention_kv4(null, null, null, null, null, null, i(1), null, null, null, null, ctypes.c_longlong(0), i(1), i(1), i(1), i(1), i(1), i(64),
+    assert lib.skv_attention_kv4(null, null, null, null, null, null, i(1), null, null, null, null, ctypes.c_longlong(0), i(1), i(1), i(1), i(1), i(64),
                                  i(16), ctypes.c_float(1.0), i(0), null) != 0
     assert b"bfloat16" in lib.skv_last_error()

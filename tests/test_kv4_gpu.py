@@ -167,7 +167,7 @@ def check_attention(heads, kv, dim, block, before, new, window=0, spread=1.0, ex
     wanted = k.attention_kv4_scratch(len(new), q.shape[0], max(new), table.shape[1], heads, kv, dim, block, window)
     scratch = torch.full((wanted,), 0xFF, dtype=torch.uint8, device="cuda")
     k.attention_kv4(q, *cache, table, ints(cu), ints(lengths), out, max(new), heads, kv, dim, block, scale, window, scratch)
-    unpacked = k._kv4_unpacked_width(len(new), max(new), table.shape[1], heads, kv, dim, block, window) > 0
+    unpacked = k._kv4_plan(len(new), max(new), table.shape[1], heads, kv, dim, block, window)[0] > 0
     for s in range(len(new)):
         ref, sums, whole = plain_kv4.attention(q[cu[s]:cu[s + 1]].double().view(new[s], heads, dim), cached(cache, table, s, lengths[s], block, 0),
                                         cached(cache, table, s, lengths[s], block, 1), before[s], scale, window)
@@ -339,13 +339,14 @@ def test_refusals():
 
     def attend(**change):
         a = dict(q=q, k_codes=cache[0], v_codes=cache[1], k_scale=cache[2], v_scale=cache[3], block_table=table, cu_q=ints([0, 1]), ctx_after=ints([40]),
-                 out=out, max_q_len=1, num_heads=4, num_kv_heads=2, head_dim=64, block_size=16, scale=0.125, window=0, scratch=None)
+                 out=out, max_q_len=1, num_heads=4, num_kv_heads=2, head_dim=64, block_size=16, scale=0.125, window=0,
+                 scratch=torch.empty(1 << 20, dtype=torch.uint8, device="cuda"))
         a.update(change)
         k.attention_kv4(**a)
 
     attend()
     for match, change in (("heads must be a positive multiple", dict(num_heads=5, q=torch.zeros(1, 320, dtype=torch.bfloat16, device="cuda"), out=torch.zeros(1, 320, dtype=torch.bfloat16, device="cuda"))),
-                          ("k_codes must be", dict(k_codes=cache[2])), ("v_scale must be torch.uint8", dict(v_scale=cache[3].float())),
+                          ("k_codes and v_codes must be", dict(k_codes=cache[2])), ("v_scale must be torch.uint8", dict(v_scale=cache[3].float())),
                           ("one length, one offset pair", dict(cu_q=ints([0, 1, 1]))), ("q and out must be", dict(out=out[:, :128].contiguous())),
                           ("a window must not be negative", dict(window=-1)), ("must be torch.bfloat16", dict(q=q.float())),
                           ("must be contiguous", dict(block_table=torch.cat([table, table], dim=1)[:, ::2])), ("CUDA tensor", dict(q=q.cpu()))):
@@ -355,6 +356,8 @@ def test_refusals():
     with pytest.raises(KernelError, match="bytes of scratch are needed"):
         attend(k_codes=long_cache[0], v_codes=long_cache[1], k_scale=long_cache[2], v_scale=long_cache[3], block_table=long_table, ctx_after=ints([4000]),
                scratch=torch.empty(8, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(KernelError, match="bytes of scratch are needed"):
+        attend(scratch=None)
     qkv = torch.zeros(1, 8 * 64, device="cuda")
     with pytest.raises(KernelError, match="width does not match"):
         k.append_kv4(qkv[:, :256].contiguous(), None, ints([0]), ints([0]), table, out, *cache, 4, 2, 64, 16)
