@@ -32,8 +32,6 @@ GATE_SIGMOID, GATE_SILU_FIRST, GATE_SILU = 0, 1, 2
 LOW_RANK_PLAIN, LOW_RANK_LOG_SIGMOID, LOW_RANK_SOFTPLUS = 0, 1, 2
 # the memories of ``matrix_step`` (csrc/channel_state.cu)
 STEP_CHANNEL, STEP_DELTA, STEP_EXP = 0, 1, 2
-# query rows a key head (heads of a group x new tokens of a sequence) up to which ``attention_kv4`` reads the 4-bit cache itself
-KV4_FEW_ROWS = 64
 KV4_SEQS = 1024            # sequences that one launch of it takes (csrc/attention_kv4.cu)
 MAX_STREAMS = 8            # copies of the residual stream that ``stream_mix`` takes (csrc/stream_mix.cu)
 
@@ -1534,6 +1532,16 @@ class Kernels:
             ctx_after.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), out_table.data_ptr(), n_seqs, k_out.shape[0] // n_seqs, num_kv_heads,
             head_dim, block_size, int(keep), _stream()), "unpack_kv4")
 
+    @staticmethod
+    def _kv4_few(max_q_len: int, group: int, positions: int) -> bool:
+        """Whether ``attention_kv4`` reads the 4-bit cache itself.  It then unpacks a key head's codes again for every 16 rows (``group`` query
+        heads of each new token), while unpacking them once for the tensor-core prompt kernel costs that kernel's whole tile of 128 queries for
+        every query head: 8 sequences of 8,000 positions, heads of 128, us, by rows of a key head: 32 heads over 8, 128 rows 168 / 241, 192 rows
+        247 / 241; 32 over 32, 48 rows 248 / 510; 32 heads of 64 over 4, 256 rows 111 / 152, 384 rows 163 / 150.  So the rows at which both take as
+        long grow with the group: 16 (2 group + 4).  Over a few hundred positions both are a chain of latencies, the prompt kernel's the shorter
+        (300 positions, 32 heads over 8 of 128: 32 rows 10.6 / 11.3, 64 rows 13.6 / 11.4)."""
+        return max_q_len * group <= (16 * (2 * group + 4) if positions > 512 else 48)
+
     def _kv4_plan(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
                   window: int) -> Tuple[int, int]:
         """How ``attention_kv4`` serves a step of these sizes: (blocks of each sequence that it reads through ``unpack_kv4``, 0
@@ -1545,7 +1553,7 @@ class Kernels:
         if plan is not None:
             return plan
         width = 0
-        if (max_q_len * (num_heads // max(1, num_kv_heads)) > KV4_FEW_ROWS and block_size & (block_size - 1) == 0 and block_size >= 16
+        if (not self._kv4_few(max_q_len, num_heads // max(1, num_kv_heads), table_width * block_size) and block_size & (block_size - 1) == 0 and block_size >= 16
                 and self.has_attention_prefill_tc() and head_dim == self.head_dim and n_seqs * -(-max_q_len // 128) <= 65535):
             width = table_width if window <= 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
         if width:

@@ -193,14 +193,15 @@ def test_attention_of_one_token_a_sequence(heads, kv, dim, block, lengths, windo
 @pytest.mark.parametrize("heads,kv,dim,block,before,new,window", [
     (8, 2, 128, 32, [0, 40, 100], [1, 3, 5], 0), (4, 4, 64, 16, [0, 7, 300], [16, 2, 9], 0), (3, 1, 80, 64, [62, 0], [5, 20], 0),
     (8, 1, 64, 64, [1000], [8], 33), (32, 8, 128, 16, [4000, 511], [5, 1], 0), (2, 1, 16, 48, [10], [70], 20), (2, 2, 208, 16, [3, 0], [9, 40], 0),
-    (4, 2, 128, 48, [90], [50], 0)])
+    (4, 2, 128, 48, [90], [50], 0), (4, 4, 128, 64, [700, 0], [96, 3], 0), (8, 1, 64, 16, [600, 10], [40, 1], 300)])
 def test_attention_of_a_few_tokens_a_sequence(heads, kv, dim, block, before, new, window):
     check_attention(heads, kv, dim, block, before, new, window)
 
 
 @pytest.mark.parametrize("heads,kv,dim,block,before,new,window", [
     (4, 2, 64, 64, [0], [300], 0), (4, 1, 128, 16, [77, 0, 900], [130, 1, 40], 0), (8, 8, 64, 32, [1000, 5], [65, 200], 100),
-    (2, 1, 128, 128, [3], [513], 64), (8, 2, 64, 64, [0] * 5, [100, 1, 64, 65, 33], 0)])
+    (2, 1, 128, 128, [3], [513], 64), (8, 2, 64, 64, [0] * 5, [100, 1, 64, 65, 33], 0), (4, 4, 128, 64, [700, 0], [97, 96], 0),
+    (8, 1, 64, 16, [600], [41], 0)])
 def test_attention_of_prompts(heads, kv, dim, block, before, new, window):
     check_attention(heads, kv, dim, block, before, new, window)
 
@@ -326,6 +327,97 @@ def test_append_read_back_and_attend_together():
             allowed = HALF_STEP * ref.abs() + (2.0 ** -8 + 2.0 ** -11) * sums
             assert bool(((out[mine].double().view(new[s], heads, dim) - ref).abs() <= allowed).all())
         before = after
+
+
+def test_cases_here_reach_both_ways_of_attending():
+    """The rule that the parametrised cases above go by: a few tokens read the cache itself, prompts the numbers it stands for."""
+    k = lib(64)
+    assert k._kv4_plan(1, 1, 100, 4, 2, 64, 64, 0)[0] == 0 and k._kv4_plan(1, 300, 5, 4, 2, 64, 64, 0)[0] == 5
+    assert k._kv4_plan(2, 200, 20, 8, 8, 64, 64, 100)[0] == min(20, (100 + 200 - 1 + 62) // 64 + 1)
+    assert k._kv4_plan(1, 300, 5, 4, 2, 64, 48, 0)[0] == 0                 # (the prompt kernel wants blocks that are powers of two)
+    assert lib(80)._kv4_plan(1, 300, 5, 4, 2, 80, 64, 0)[0] == 0           # (and heads of 64 or 128)
+
+
+@pytest.mark.parametrize("new", [[0, 1, 0, 1], [3, 0, 0, 2]])
+def test_sequences_without_new_tokens(new):
+    """They have no rows, and nothing of their cache is read."""
+    k = lib(64)
+    before = [100, 700, 40, 300]
+    cache, table = make_cache(2, 64, 16, [b + n for b, n in zip(before, new)])
+    q = torch.randn(sum(new), 4 * 64, device="cuda").bfloat16()
+    cu = [0]
+    for c in new:
+        cu.append(cu[-1] + c)
+    got = run_step(k, q, cache, table, cu, [b + n for b, n in zip(before, new)], 4, 2, 64, 16, max(new))
+    for s in range(4):
+        if new[s]:
+            alone = run_step(k, q[cu[s]:cu[s + 1]].contiguous(), cache, table[s:s + 1].contiguous(), [0, new[s]], [before[s] + new[s]], 4, 2, 64, 16, new[s])
+            torch.testing.assert_close(got[cu[s]:cu[s + 1]].float(), alone.float(), rtol=2 * HALF_STEP, atol=2.0 ** -10)
+
+
+@pytest.mark.parametrize("n_seqs,most", [(1100, 1), (2051, 2)])
+def test_more_sequences_than_a_launch_takes(n_seqs, most):
+    k = lib(64)
+    lengths = [1 + (7 * i) % 40 + most for i in range(n_seqs)]
+    cache, table = make_cache(1, 64, 16, [max(lengths)] * 3)
+    table = table[torch.arange(n_seqs, device="cuda") % 3].contiguous()    # (three caches, many readers)
+    q = torch.randn(n_seqs * most, 2 * 64, device="cuda").bfloat16()
+    got = run_step(k, q, cache, table, [most * i for i in range(n_seqs + 1)], lengths, 2, 1, 64, 16, most)
+    for s in (0, 1, 1023, 1024, 1025, n_seqs - 1):
+        mine = slice(most * s, most * (s + 1))
+        ref, sums, _ = plain_kv4.attention(q[mine].double().view(most, 2, 64), cached(cache, table, s, lengths[s], 16, 0),
+                                           cached(cache, table, s, lengths[s], 16, 1), lengths[s] - most, 0.125)
+        assert bool(((got[mine].double().view(most, 2, 64) - ref).abs() <= HALF_STEP * ref.abs() + 2.0 ** -10 * sums).all())
+
+
+def test_a_captured_step_follows_its_inputs():
+    """A replayed graph reads lengths, tables and rows as they are then; two graphs with a scratch each, on another stream than the capture's."""
+    k = lib(128)
+    heads, kv, dim, block = 8, 2, 128, 32
+    cache, table = make_cache(kv, dim, block, [2000, 900])
+    q = torch.randn(2, heads * dim, device="cuda").bfloat16()
+    ctx, cu = ints([1500, 300]), ints([0, 1, 2])
+    wanted = k.attention_kv4_scratch(2, 2, 1, table.shape[1], heads, kv, dim, block)
+    graphs = []
+    for _ in range(2):
+        out, scratch = torch.empty_like(q), torch.empty(wanted, dtype=torch.uint8, device="cuda")
+        call = lambda: k.attention_kv4(q, *cache, table, cu, ctx, out, 1, heads, kv, dim, block, dim ** -0.5, 0, scratch)
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        graphs.append((graph, out, scratch))
+    side = torch.cuda.Stream()
+    for lengths in ([1500, 300], [2000, 1], [33, 900]):
+        ctx.copy_(ints(lengths))
+        q.normal_()
+        torch.cuda.synchronize()
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        eager = torch.empty_like(q)
+        k.attention_kv4(q, *cache, table, cu, ctx, eager, 1, heads, kv, dim, block, dim ** -0.5, 0, torch.empty(wanted, dtype=torch.uint8, device="cuda"))
+        assert torch.equal(graphs[0][1], eager) and torch.equal(graphs[1][1], eager)
+        for s, length in enumerate(lengths):
+            ref, sums, _ = plain_kv4.attention(q[s:s + 1].double().view(1, heads, dim), cached(cache, table, s, length, block, 0),
+                                               cached(cache, table, s, length, block, 1), length - 1, dim ** -0.5)
+            assert bool(((eager[s:s + 1].double().view(1, heads, dim) - ref).abs() <= HALF_STEP * ref.abs() + 2.0 ** -10 * sums).all())
+
+
+def test_another_device_than_the_current_one_is_refused(monkeypatch):
+    from stratakv_b200.ops import KernelError
+    k = lib(64)
+    cache, table = make_cache(1, 64, 16, [20])
+    q = torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda")
+    run_step(k, q, cache, table, [0, 1], [20], 1, 1, 64, 16, 1)
+    current = torch.cuda.current_device()
+    scratch = torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    cu, ctx = ints([0, 1]), ints([20])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current + 1)
+    with pytest.raises(KernelError, match="another device"):
+        k.attention_kv4(q, *cache, table, cu, ctx, q.clone(), 1, 1, 1, 64, 16, 0.125, 0, scratch)
 
 
 # ---- refusals -----------------------------------------------------------------------------------------------------------
