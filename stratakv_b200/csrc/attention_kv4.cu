@@ -100,6 +100,10 @@ __device__ __forceinline__ float part_weight(float m, float top) { return m == -
 struct Kv4Cut {
     int n_seqs, num_heads, num_kv_heads, window, least;     // a run has at least `least` chunks
     int most_positions, most_tiles;                         // what the call has room for
+    int group;                                              // query heads of a key head, and 2^32 / group, rounded up
+    uint32_t group_magic;
+    // x / group, as the upper half of a product (exact while x * group stays below 2^32)
+    __device__ __forceinline__ int of_group(int x) const { return group == 1 ? x : (int)__umulhi((uint32_t)x, group_magic); }
 };
 struct Kv4Share {
     int q_begin, q_len, ctx, tiles, first_chunk, chunks;    // chunks of an item
@@ -112,7 +116,7 @@ __device__ __forceinline__ Kv4Share kv4_share(const Kv4Cut& cut, const int* cu_q
     s.q_begin = cu_q[seq];
     s.q_len = cu_q[seq + 1] - s.q_begin;
     s.ctx = min(ctx_after[seq], cut.most_positions);
-    s.tiles = min((s.q_len * (cut.num_heads / cut.num_kv_heads) + ROWS - 1) / ROWS, cut.most_tiles);
+    s.tiles = min((s.q_len * cut.group + ROWS - 1) / ROWS, cut.most_tiles);
     s.first_chunk = cut.window > 0 ? max(0, s.ctx - s.q_len - cut.window + 1) / CK : 0;
     s.chunks = s.q_len > 0 ? (s.ctx + CK - 1) / CK - s.first_chunk : 0;
     return s;
@@ -126,19 +130,28 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
                      float4* __restrict__ partial_o, float2* __restrict__ partial_ml, const Kv4Cut cut, int block_size, float scale,
                      uint32_t chunks_magic, uint32_t ones) {
     extern __shared__ __align__(16) uint8_t kv4_smem[];
-    __shared__ int upto[KV4_SEQS], warp_all[KV4_WARPS];     // chunks up to and with a sequence; of a warp's sequences
+    __shared__ int upto_all[KV4_SEQS], warp_all[KV4_WARPS];
     constexpr int ROWS = 8 * NT;
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int num_heads = cut.num_heads, num_kv_heads = cut.num_kv_heads, window = cut.window, group = num_heads / num_kv_heads;
+    const int num_heads = cut.num_heads, num_kv_heads = cut.num_kv_heads, window = cut.window, group = cut.group;
     int total = 0;
+    // upto[s]: the chunks up to and with sequence s.  Up to 32 sequences every warp adds up by itself, which needs no barrier.
+    const bool few = cut.n_seqs <= 32;
+    const int* upto = few ? upto_all + 32 * warp : upto_all;
     for (int s0 = 0; s0 < cut.n_seqs; s0 += KV4_WARPS * 32) {
-        int sum = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, s0 + threadIdx.x).all(cut);
+        int sum = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, s0 + (few ? lane : (int)threadIdx.x)).all(cut);
 #pragma unroll
         for (int o2 = 1; o2 < 32; o2 *= 2) {
             const int before = __shfl_up_sync(0xffffffffu, sum, o2);
             if (lane >= o2) sum += before;
+        }
+        if (few) {
+            upto_all[32 * warp + lane] = sum;
+            total = __shfl_sync(0xffffffffu, sum, 31);
+            __syncwarp();
+            break;
         }
         if (lane == 31) warp_all[warp] = sum;
         __syncthreads();
@@ -146,9 +159,9 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
             const int v = warp_all[w];
             if (w < warp) sum += v;
         }
-        if (s0 + threadIdx.x < cut.n_seqs) upto[s0 + threadIdx.x] = total + sum;
+        if (s0 + threadIdx.x < cut.n_seqs) upto_all[s0 + threadIdx.x] = total + sum;
         __syncthreads();
-        total = upto[min(s0 + KV4_WARPS * 32, cut.n_seqs) - 1];
+        total = upto_all[min(s0 + KV4_WARPS * 32, cut.n_seqs) - 1];
     }
     const int workers = (int)gridDim.x * KV4_WARPS, run = max(cut.least, (total + workers - 1) / workers);
     const int worker = blockIdx.x + gridDim.x * warp;       // (runs that follow each other lie on different SMs)
@@ -156,7 +169,7 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     if (run_begin >= total) return;
     const int run_end = (int)min((long long)total, run_begin + run);
     int seq = 0;                                            // the first whose chunks reach beyond run_begin
-    for (int step = KV4_SEQS / 2; step > 0; step /= 2)
+    for (int step = few ? 16 : KV4_SEQS / 2; step > 0; step /= 2)
         if (seq + step <= cut.n_seqs && upto[seq + step - 1] <= (int)run_begin) seq += step;
 
     for (int done = (int)run_begin; done < run_end;) {
@@ -170,9 +183,22 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     done += count;
     const int row0 = (item - kv_head * tiles) * ROWS, rows = q_len * group, before = share.ctx - q_len;
     const int last_query = min(rows, row0 + ROWS) - 1;
-    const int end = before + last_query / group + 1;                        // keys that any row of the tile sees lie before it
+    const int end = before + cut.of_group(last_query) + 1;                        // keys that any row of the tile sees lie before it
     const int my_first = share.first_chunk + from, my_end = min(my_first + count, (end + CK - 1) / CK);
     const int* table = block_table + (size_t)seq * table_width;
+
+    // Queries on their way: lane (g, t) has a quarter of row g of each tile of eight.
+    uint4 raw[NT][KWORDS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = row0 + 8 * n + g, token = cut.of_group(min(r, rows - 1));
+        const __nv_bfloat16* at = q + ((size_t)(q_begin + token) * num_heads + kv_head * group + min(r, rows - 1) - token * group) * FHD;
+#pragma unroll
+        for (int j = 0; j < KWORDS; ++j) {
+            const int d = t * (FPAD / 4) + 8 * j;
+            raw[n][j] = r < rows && d < FHD ? *(const uint4*)(at + d) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
 
     // Copies of a chunk: pieces of 16 bytes, a lane one after the other.
     constexpr int CHUNK_BYTES = CHUNK_OF<CK>, PIECES = FHD % 32 ? 1 : FHD / 32;      // (of a row)
@@ -223,28 +249,22 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
         block = following;
     }
 
-    // Queries: lane (g, t) has a quarter of row g of each tile of eight; word j's codes p and p + 4 meet numbers 8j + p and 8j + p + 4.
+    // Queries as halves: word j's codes p and p + 4 meet numbers 8j + p and 8j + p + 4.
     uint32_t qb[NT][KSTEP4][2];
-    float2 factor[NT];                              // of rows 2t and 2t + 1: scale * log2 e * the power of two taken off the query
+    float2 factor[NT];                                // of rows 2t and 2t + 1: scale * log2 e * the power of two taken off the query
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = row0 + 8 * n + g;
-        const __nv_bfloat16* at = q + ((size_t)(q_begin + min(r, rows - 1) / group) * num_heads + kv_head * group + min(r, rows - 1) % group) * FHD;
-        uint4 raw[KWORDS];
         float most = 0.0f;
         bool finite = true;
 #pragma unroll
-        for (int j = 0; j < KWORDS; ++j) {
-            const int d = t * (FPAD / 4) + 8 * j;
-            raw[j] = r < rows && d < FHD ? *(const uint4*)(at + d) : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < KWORDS; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t w = (&raw[j].x)[e];
+                const uint32_t w = (&raw[n][j].x)[e];
                 const float a = __uint_as_float(w << 16), b = __uint_as_float(w & 0xffff0000u);
                 most = fmaxf(most, fmaxf(fabsf(a), fabsf(b)));
                 finite = finite && isfinite(a) && isfinite(b);
             }
-        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         finite = (__ballot_sync(0xffffffffu, finite) >> (lane & 28) & 15u) == 15u;
@@ -256,7 +276,7 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
             float x[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t w = (&raw[j].x)[e];
+                const uint32_t w = (&raw[n][j].x)[e];
                 x[2 * e] = __uint_as_float(w << 16) * down;
                 x[2 * e + 1] = __uint_as_float(w & 0xffff0000u) * down;
             }
@@ -289,18 +309,18 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int r = row0 + 8 * n + 2 * t + c;
-                    position[n][c] = r < rows ? before + r / group : -1;
+                    position[n][c] = r < rows ? before + cut.of_group(r) : -1;
                 }
         }
-        // S^T: keys of indices g, g + 8 by rows 2t, 2t + 1.  Two sums take turns: an instruction that adds to the one before it would wait for it.
-        float s[HALVES][NT][4], other[HALVES][NT][4];
+        // S^T: keys of indices g, g + 8 by rows 2t, 2t + 1
+        float s[HALVES][NT][4];
         uint32_t kw[HALVES][2][KWORDS];
 #pragma unroll
         for (int h16 = 0; h16 < HALVES; ++h16) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[h16][n][c] = other[h16][n][c] = 0.0f;
+                for (int c = 0; c < 4; ++c) s[h16][n][c] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -317,9 +337,9 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
                 }
         }
 #pragma unroll
-        for (int j = 0; j < KWORDS; j += 2)
+        for (int h16 = 0; h16 < HALVES; ++h16)
 #pragma unroll
-            for (int h16 = 0; h16 < HALVES; ++h16) {
+            for (int j = 0; j < KWORDS; j += 2) {
                 const bool there = FHD == FPAD || t * (FPAD / 4) + 8 * j < FHD;
                 Kv4Scale of[2];
 #pragma unroll
@@ -333,19 +353,10 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma_f16_16816(s[h16][n], a[0][0], a[1][0], a[0][1], a[1][1], qb[n][2 * (j + w)][0], qb[n][2 * (j + w)][1]);
-                        mma_f16_16816(other[h16][n], a[0][2], a[1][2], a[0][3], a[1][3], qb[n][2 * (j + w) + 1][0], qb[n][2 * (j + w) + 1][1]);
+                        mma_f16_16816(s[h16][n], a[0][2], a[1][2], a[0][3], a[1][3], qb[n][2 * (j + w) + 1][0], qb[n][2 * (j + w) + 1][1]);
                     }
                 }
             }
-#pragma unroll
-        for (int h16 = 0; h16 < HALVES; ++h16)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    const float2 v = add2(make_float2(s[h16][n][c], s[h16][n][c + 1]), make_float2(other[h16][n][c], other[h16][n][c + 1]));
-                    s[h16][n][c] = v.x; s[h16][n][c + 1] = v.y;
-                }
         auto sees = [&](int h16, int n, int c) {
             const int key = j0 + 16 * h16 + key_of_index(g) + 8 * (c >> 1), pos = position[n][c & 1];
             return key <= pos && (window == 0 || key > pos - window);
@@ -483,7 +494,7 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     };
 
     // every row of the block sees keys all_from .. all_to - 1
-    const int all_to = before + row0 / group + 1, all_from = window > 0 ? max(0, before + last_query / group - window + 1) : 0;
+    const int all_to = before + cut.of_group(row0) + 1, all_from = window > 0 ? max(0, before + cut.of_group(last_query) - window + 1) : 0;
     int stage = 0, free_stage = KV4_STAGES - 1;
     for (int at = my_first; at < my_end; ++at) {
         ring_wait<KV4_STAGES - 2>();
@@ -523,7 +534,8 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
             for (int c = 0; c < 2; ++c) {
                 const int r = row0 + 8 * n + 2 * t + c;
                 if (r >= rows) continue;
-                __nv_bfloat16* to = out + ((size_t)(q_begin + r / group) * num_heads + kv_head * group + r % group) * FHD;
+                const int token = cut.of_group(r);
+                __nv_bfloat16* to = out + ((size_t)(q_begin + token) * num_heads + kv_head * group + r - token * group) * FHD;
                 const float by = 1.0f / (c ? sum[n].y : sum[n].x);
 #pragma unroll
                 for (int j = 0; j < OTILE4; ++j) {
@@ -549,7 +561,7 @@ kv4_merge_kernel(const float4* __restrict__ partial_o, const float4* __restrict_
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int of_seq = cut.num_kv_heads * cut.most_tiles, seq = blockIdx.x / of_seq, item = blockIdx.x - seq * of_seq;
-    const int kv_head = item / cut.most_tiles, at_tile = item - kv_head * cut.most_tiles, group = cut.num_heads / cut.num_kv_heads;
+    const int kv_head = item / cut.most_tiles, at_tile = item - kv_head * cut.most_tiles, group = cut.group;
     const Kv4Share share = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, seq);
     int total = 0, base = 0;                          // chunks of all sequences, and of those before this one
     for (int s = threadIdx.x; s < cut.n_seqs; s += KV4_WARPS * 32) {
@@ -617,8 +629,9 @@ kv4_merge_kernel(const float4* __restrict__ partial_o, const float4* __restrict_
         for (int c = 0; c < 2; ++c) {
             const int r = at_tile * ROWS + 8 * n + 2 * t + c;
             if (r >= share.q_len * group) continue;
+            const int token = cut.of_group(r);
             const float by = 1.0f / (c ? sum.y : sum.x);
-            *(__nv_bfloat162*)(out + ((size_t)(share.q_begin + r / group) * cut.num_heads + kv_head * group + r % group) * FHD + d) =
+            *(__nv_bfloat162*)(out + ((size_t)(share.q_begin + token) * cut.num_heads + kv_head * group + r - token * group) * FHD + d) =
                 __floats2bfloat162_rn((c ? acc.y : acc.x) * by, (c ? acc.w : acc.z) * by);
         }
     }
@@ -646,7 +659,8 @@ static Kv4Plan kv4_plan(int n_seqs, int max_q_len, int table_width, int num_head
     const long long wanted = (plan.chunks + least - 1) / least;
     plan.blocks = (int)(wanted < resident ? wanted : resident);
     const long long workers = (long long)plan.blocks * KV4_WARPS, run = plan.chunks / workers > least ? plan.chunks / workers : least;
-    plan.cut = {n_seqs, num_heads, num_kv_heads, window, least, (int)most, row_tiles};
+    const uint32_t group = (uint32_t)(num_heads / num_kv_heads);
+    plan.cut = {n_seqs, num_heads, num_kv_heads, window, least, (int)most, row_tiles, (int)group, (uint32_t)((0x100000000ull + group - 1) / group)};
     plan.parts = chunks > 1 ? (chunks + run - 1) / run + 1 : 1;
     plan.floats = plan.parts > 1 ? 2 * workers * 8 * plan.tiles_of_8 * (FPAD + 2) : 0;
     return plan;
@@ -702,7 +716,7 @@ SKV_EXPORT int skv_attention_kv4(const void* q, const void* k_codes, const void*
         return fail("skv_attention_kv4", "the block table spans too many positions for blocks of this size");
     if (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)out | (uintptr_t)scratch) & 15)
         return fail("skv_attention_kv4", "operands must be 16-byte aligned");
-    if ((long long)n_seqs * max_q_len * num_heads > 0x3fffffffLL) return fail("skv_attention_kv4", "too many rows in one step");
+    if ((long long)n_seqs * max_q_len * num_heads > 0x3fffffffLL || (long long)(max_q_len + 16) * num_heads * (num_heads / num_kv_heads) > 0xffffffffLL) return fail("skv_attention_kv4", "too many rows in one step");
     const Kv4Plan plan = kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window, sm_count());
     if (plan.chunks > 0x7fffffffLL) return fail("skv_attention_kv4", "too many rows and positions in one step");
     if (plan.floats && (!scratch || scratch_floats < plan.floats)) return fail("skv_attention_kv4", "scratch is too small");
