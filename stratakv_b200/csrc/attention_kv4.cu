@@ -695,7 +695,10 @@ using namespace skv;
 // Floats of scratch that a call of these sizes needs (0: none).
 SKV_EXPORT long long skv_attention_kv4_scratch(int n_seqs, int max_q_len, int table_width, int num_heads, int num_kv_heads, int block_size,
                                                int window) {
-    if (n_seqs <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || block_size <= 0) return 0;
+    // (sizes that skv_attention_kv4 does nothing for, or refuses)
+    if (n_seqs <= 0 || max_q_len <= 0 || table_width <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || block_size <= 0 ||
+        block_size % 16 != 0 || window < 0)
+        return 0;
     return kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window, sm_count()).floats;
 }
 

@@ -147,6 +147,19 @@ def test_the_libraries_refuse_bad_sizes():
         assert code != 0 and match in message, (changes, message)
 
 
+def scratch_of(lib, seqs=1, most=1, width=4, heads=4, kv=2, block=16, window=0):
+    lib.skv_attention_kv4_scratch.restype = ctypes.c_longlong
+    return lib.skv_attention_kv4_scratch(*(ctypes.c_int(n) for n in (seqs, most, width, heads, kv, block, window)))
+
+
+def test_scratch_of_sizes_that_are_refused():
+    lib = library("bfloat16", 64)
+    assert scratch_of(lib) > 0
+    for changes in (dict(width=0), dict(width=-1), dict(block=8, width=1), dict(block=0), dict(block=24), dict(heads=3), dict(heads=0), dict(kv=0),
+                    dict(seqs=0), dict(most=0), dict(window=-1)):
+        assert scratch_of(lib, **changes) == 0, changes
+
+
 def test_float32_libraries_have_none():
     lib = library("float32", 64)
     null, i = ctypes.c_void_p(0), ctypes.c_int
