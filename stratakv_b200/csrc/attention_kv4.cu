@@ -651,7 +651,9 @@ static Kv4Plan kv4_plan(int n_seqs, int max_q_len, int table_width, int num_head
     plan.tiles_of_8 = rows > 8 ? 2 : 1;
     plan.chunk = block_size % 32 == 0 ? 32 : 16;
     const int row_tiles = (int)((rows + 8 * plan.tiles_of_8 - 1) / (8 * plan.tiles_of_8));
-    const long long most = (long long)table_width * block_size, span = window > 0 && window + max_q_len - 1 < most ? window + max_q_len - 1 : most;
+    const long long most = (long long)table_width * block_size;
+    if (window >= most) window = 0;                   // (one that no position can leave: sums of it and a length could pass 32 bits)
+    const long long span = window > 0 && (long long)window + max_q_len - 1 < most ? (long long)window + max_q_len - 1 : most;
     const long long chunks = span < most ? (span + plan.chunk - 2) / plan.chunk + 1 : most / plan.chunk;       // of an item
     plan.items = (long long)n_seqs * num_kv_heads * row_tiles;
     plan.chunks = plan.items * chunks;
@@ -716,7 +718,7 @@ SKV_EXPORT int skv_attention_kv4(const void* q, const void* k_codes, const void*
     if (block_size <= 0 || block_size % 16 != 0) return fail("skv_attention_kv4", "block_size must be a positive multiple of 16");
     if (window < 0) return fail("skv_attention_kv4", "a window must not be negative");
     if ((unsigned long long)num_kv_heads * block_size * FHD > 0x80000000ull) return fail("skv_attention_kv4", "a cache block is too large (2 GB at most)");
-    if ((unsigned long long)table_width * (block_size / 16) * (block_size / 16) >= 0x100000000ull || (unsigned long long)table_width * block_size > 0x7fffffffull)
+    if ((unsigned long long)table_width * (block_size / 16) * (block_size / 16) >= 0x100000000ull || (unsigned long long)table_width * block_size > 0x7fffff00ull)
         return fail("skv_attention_kv4", "the block table spans too many positions for blocks of this size");
     if (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scale | (uintptr_t)v_scale | (uintptr_t)out | (uintptr_t)scratch) & 15)
         return fail("skv_attention_kv4", "operands must be 16-byte aligned");

@@ -1543,19 +1543,23 @@ class Kernels:
         return max_q_len * group <= (16 * (2 * group + 4) if positions > 512 else 48)
 
     def _kv4_plan(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
-                  window: int) -> Tuple[int, int]:
+                  window: int) -> Tuple[int, int, int]:
         """How ``attention_kv4`` serves a step of these sizes: (blocks of each sequence that it reads through ``unpack_kv4``, 0
-        where it reads the 4-bit cache itself; bytes of scratch)."""
+        where it reads the 4-bit cache itself; bytes of scratch; the window, 0 for one that the table's positions cannot leave)."""
         if not self._kv4_prototyped:
             self._kv4_prototypes()
         key = (n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
         plan = self._kv4_plans.get(key)
         if plan is not None:
             return plan
+        if window < 0:
+            raise KernelError("attention_kv4: a window must not be negative")
+        if window >= table_width * block_size:
+            window = 0
         width = 0
         if (not self._kv4_few(max_q_len, num_heads // max(1, num_kv_heads), table_width * block_size) and block_size & (block_size - 1) == 0 and block_size >= 16
                 and self.has_attention_prefill_tc() and head_dim == self.head_dim and n_seqs * -(-max_q_len // 128) <= 65535):
-            width = table_width if window <= 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
+            width = table_width if window == 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
         if width:
             wanted = 4 * n_seqs * width * num_kv_heads * block_size * head_dim + 4 * n_seqs * table_width
         else:
@@ -1563,8 +1567,8 @@ class Kernels:
                                                             block_size, window)
         if len(self._kv4_plans) > 4096:
             self._kv4_plans.clear()
-        self._kv4_plans[key] = (width, wanted)
-        return width, wanted
+        self._kv4_plans[key] = (width, wanted, window)
+        return width, wanted, window
 
     def attention_kv4_scratch(self, n_seqs: int, n_tokens: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int,
                               head_dim: int, block_size: int, window: int = 0) -> int:
@@ -1588,7 +1592,7 @@ class Kernels:
             raise KernelError("attention_kv4: one length, one offset pair and one table row per sequence is needed")
         if q.shape != (n, num_heads * head_dim) or out.shape != q.shape or max_q_len < 1:
             raise KernelError("attention_kv4: q and out must be [tokens, heads * head_dim]")
-        width, wanted = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
+        width, wanted, window = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
         if wanted:
             if scratch is None or scratch.numel() < wanted:
                 raise KernelError(f"attention_kv4: {wanted} bytes of scratch are needed, not {0 if scratch is None else scratch.numel()}")

@@ -160,6 +160,13 @@ def test_scratch_of_sizes_that_are_refused():
         assert scratch_of(lib, **changes) == 0, changes
 
 
+def test_a_window_that_no_position_can_leave_is_none():
+    lib = library("bfloat16", 64)
+    for most in (1, 5, 300):
+        for window in (64, 1000, 2 ** 31 - 1):
+            assert scratch_of(lib, most=most, window=window) == scratch_of(lib, most=most) > 0
+
+
 def test_float32_libraries_have_none():
     lib = library("float32", 64)
     null, i = ctypes.c_void_p(0), ctypes.c_int

@@ -266,6 +266,31 @@ def test_a_query_that_is_not_finite_gives_nan_and_spoils_no_other(bad):
     assert torch.equal(got, clean)
 
 
+def twice_off(cache, unpacked):
+    """How far two results over this cache may lie apart before they are rounded: each is off by the roundings of its probabilities and its
+    sums (see check_attention) times the largest value."""
+    values = plain_kv4.read(cache[1], cache[3])
+    return 2 * ((2.0 ** -8 if unpacked else 2.0 ** -11) + 2.0 ** -11) * float(values[~torch.isnan(values)].abs().max())
+
+
+@pytest.mark.parametrize("new", [1, 4, 200])
+def test_windows_of_any_size(new):
+    """One as long as what is cached, or longer, changes nothing; a negative one is refused, whichever way the step takes."""
+    from stratakv_b200.ops import KernelError
+    k = lib(64)
+    cache, table = make_cache(2, 64, 16, [300 + new])
+    q = torch.randn(new, 4 * 64, device="cuda").bfloat16()
+    plain = run_step(k, q, cache, table, [0, new], [300 + new], 4, 2, 64, 16, new)
+    for window in (300 + new, 10 ** 6, 2 ** 31 - new, 2 ** 31 - 1, 2 ** 32 + 5):
+        got = run_step(k, q, cache, table, [0, new], [300 + new], 4, 2, 64, 16, new, window=window)
+        if window < table.numel() * 16:                    # (one that the table could leave is cut as windows are: sums in another order)
+            torch.testing.assert_close(got.float(), plain.float(), rtol=2 * HALF_STEP, atol=twice_off(cache, new == 200))
+        else:
+            assert torch.equal(got, plain), window
+    with pytest.raises(KernelError, match="must not be negative"):
+        run_step(k, q, cache, table, [0, new], [300 + new], 4, 2, 64, 16, new, window=-1)
+
+
 def test_queries_of_any_size():
     """Powers of two on a query and off the scale change nothing but the products' exponents."""
     k = lib(128)
