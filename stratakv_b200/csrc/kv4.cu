@@ -194,7 +194,8 @@ SKV_EXPORT int skv_append_kv4(const float* qkv, const float* cos_sin, const int*
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
         return fail("skv_append_kv4", "heads must be a positive multiple of kv heads");
     if (block_size <= 0 || block_size % 16 != 0) return fail("skv_append_kv4", "block_size must be a positive multiple of 16");
-    if (((uintptr_t)qkv | (uintptr_t)cos_sin | (uintptr_t)q_out) & 15) return fail("skv_append_kv4", "operands must be 16-byte aligned");
+    if (((uintptr_t)qkv | (uintptr_t)cos_sin | (uintptr_t)q_out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scale | (uintptr_t)v_scale) & 15)
+        return fail("skv_append_kv4", "operands must be 16-byte aligned");
     // twice four numbers a thread, or four
     const bool paired = head_dim % 32 == 0;
     const long long items = (long long)(num_heads + (write_kv ? 2 * num_kv_heads : 0)) * (head_dim / (paired ? 8 : 4));

@@ -147,6 +147,16 @@ def test_the_libraries_refuse_bad_sizes():
         assert code != 0 and match in message, (changes, message)
 
 
+def test_append_refuses_a_cache_that_no_reader_takes():
+    """Codes are stored two bytes at a time, and read 16 bytes at a time."""
+    lib = library("bfloat16", 64)
+    null, i = ctypes.c_void_p(0), ctypes.c_int
+    for which in range(4):
+        cache = [ctypes.c_void_p(1 if of == which else 0) for of in range(4)]
+        assert lib.skv_append_kv4(null, null, null, null, null, i(1), null, *cache, i(1), i(4), i(2), i(64), i(16), i(1), null) != 0
+        assert b"aligned" in lib.skv_last_error()
+
+
 def scratch_of(lib, seqs=1, most=1, width=4, heads=4, kv=2, block=16, window=0):
     lib.skv_attention_kv4_scratch.restype = ctypes.c_longlong
     return lib.skv_attention_kv4_scratch(*(ctypes.c_int(n) for n in (seqs, most, width, heads, kv, block, window)))
