@@ -99,7 +99,7 @@ __device__ __forceinline__ float part_weight(float m, float top) { return m == -
 // against 73.9, 12 ragged sequences of 32 key heads 52.4 against 46.4.)
 struct Kv4Cut {
     int n_seqs, num_heads, num_kv_heads, window, least;     // a run has at least `least` chunks
-    int most_positions, most_tiles;                         // what the call has room for
+    int most_positions, most_new, most_tiles;               // what the call has room for: lengths beyond it are cut
     int group;                                              // query heads of a key head, and 2^32 / group, rounded up
     uint32_t group_magic;
     // x / group, as the upper half of a product (exact while x * group stays below 2^32)
@@ -114,9 +114,9 @@ __device__ __forceinline__ Kv4Share kv4_share(const Kv4Cut& cut, const int* cu_q
     Kv4Share s = {};
     if (seq >= cut.n_seqs) return s;
     s.q_begin = cu_q[seq];
-    s.q_len = cu_q[seq + 1] - s.q_begin;
-    s.ctx = min(ctx_after[seq], cut.most_positions);
-    s.tiles = min((s.q_len * cut.group + ROWS - 1) / ROWS, cut.most_tiles);
+    s.q_len = min(cu_q[seq + 1] - s.q_begin, cut.most_new);
+    s.ctx = max(0, min(ctx_after[seq], cut.most_positions));
+    s.tiles = (s.q_len * cut.group + ROWS - 1) / ROWS;
     s.first_chunk = cut.window > 0 ? max(0, s.ctx - s.q_len - cut.window + 1) / CK : 0;
     s.chunks = s.q_len > 0 ? (s.ctx + CK - 1) / CK - s.first_chunk : 0;
     return s;
@@ -663,7 +663,7 @@ static Kv4Plan kv4_plan(int n_seqs, int max_q_len, int table_width, int num_head
     plan.blocks = (int)(wanted < resident ? wanted : resident);
     const long long workers = (long long)plan.blocks * KV4_WARPS, run = plan.chunks / workers > least ? plan.chunks / workers : least;
     const uint32_t group = (uint32_t)(num_heads / num_kv_heads);
-    plan.cut = {n_seqs, num_heads, num_kv_heads, window, least, (int)most, row_tiles, (int)group, (uint32_t)((0x100000000ull + group - 1) / group)};
+    plan.cut = {n_seqs, num_heads, num_kv_heads, window, least, (int)most, max_q_len, row_tiles, (int)group, (uint32_t)((0x100000000ull + group - 1) / group)};
     plan.parts = chunks > 1 ? (chunks + run - 1) / run + 1 : 1;
     plan.floats = plan.parts > 1 ? 2 * workers * 8 * plan.tiles_of_8 * (FPAD + 2) : 0;
     return plan;

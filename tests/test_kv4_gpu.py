@@ -380,6 +380,19 @@ def test_sequences_without_new_tokens(new):
             torch.testing.assert_close(got[cu[s]:cu[s + 1]].float(), alone.float(), rtol=2 * HALF_STEP, atol=2.0 ** -10)
 
 
+def test_lengths_that_contradict_the_call_spoil_no_other_sequence():
+    """More new tokens than the call's maximum, a negative length, one beyond the table: that sequence's rows are anyone's guess."""
+    k = lib(64)
+    cache, table = make_cache(2, 64, 16, [90, 90, 90, 90, 90, 90])
+    q = torch.randn(8, 4 * 64, device="cuda").bfloat16()
+    cu, ctx = [0, 1, 4, 5, 6, 7, 8], [90, 90, -5, 33, 10 ** 6, 70]
+    for window in (0, 1, 20):
+        got = run_step(k, q, cache, table, cu, ctx, 4, 2, 64, 16, 1, window=window)
+        for s in (0, 3, 5):
+            alone = run_step(k, q[cu[s]:cu[s] + 1].contiguous(), cache, table[s:s + 1].contiguous(), [0, 1], [ctx[s]], 4, 2, 64, 16, 1, window=window)
+            torch.testing.assert_close(got[cu[s]].float(), alone[0].float(), rtol=2 * HALF_STEP, atol=twice_off(cache, False))
+
+
 @pytest.mark.parametrize("n_seqs,most", [(1100, 1), (2051, 2)])
 def test_more_sequences_than_a_launch_takes(n_seqs, most):
     k = lib(64)
