@@ -33,6 +33,7 @@ LOW_RANK_PLAIN, LOW_RANK_LOG_SIGMOID, LOW_RANK_SOFTPLUS = 0, 1, 2
 # the memories of ``matrix_step`` (csrc/channel_state.cu)
 STEP_CHANNEL, STEP_DELTA, STEP_EXP = 0, 1, 2
 KV4_SEQS = 1024            # sequences that one launch of it takes (csrc/attention_kv4.cu)
+KV4_UNPACKED = 1 << 30     # bytes of a 4-bit cache's sequences that are read back at once (or one sequence's, if those are more)
 MAX_STREAMS = 8            # copies of the residual stream that ``stream_mix`` takes (csrc/stream_mix.cu)
 
 
@@ -1543,9 +1544,10 @@ class Kernels:
         return max_q_len * group <= (16 * (2 * group + 4) if positions > 512 else 48)
 
     def _kv4_plan(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
-                  window: int) -> Tuple[int, int, int]:
+                  window: int) -> Tuple[int, int, int, int]:
         """How ``attention_kv4`` serves a step of these sizes: (blocks of each sequence that it reads through ``unpack_kv4``, 0
-        where it reads the 4-bit cache itself; bytes of scratch; the window, 0 for one that the table's positions cannot leave)."""
+        where it reads the 4-bit cache itself; bytes of scratch; the window, 0 for one that the table's positions cannot leave;
+        sequences that it takes at once)."""
         if not self._kv4_prototyped:
             self._kv4_prototypes()
         key = (n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
@@ -1556,19 +1558,22 @@ class Kernels:
             raise KernelError("attention_kv4: a window must not be negative")
         if window >= table_width * block_size:
             window = 0
-        width = 0
+        width, at_once, tiles = 0, min(n_seqs, KV4_SEQS), -(-max_q_len // 128)
         if (not self._kv4_few(max_q_len, num_heads // max(1, num_kv_heads), table_width * block_size) and block_size & (block_size - 1) == 0 and block_size >= 16
-                and self.has_attention_prefill_tc() and head_dim == self.head_dim and n_seqs * -(-max_q_len // 128) <= 65535):
+                and self.has_attention_prefill_tc() and head_dim == self.head_dim and tiles <= 65535):
             width = table_width if window == 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
         if width:
-            wanted = 4 * n_seqs * width * num_kv_heads * block_size * head_dim + 4 * n_seqs * table_width
+            # every sequence has room for the longest: a long one among many short ones must not ask for many times the cache
+            each = 4 * width * num_kv_heads * block_size * head_dim + 4 * table_width
+            at_once = max(1, min(n_seqs, KV4_UNPACKED // each, 65535 // tiles))
+            wanted = min(n_seqs, at_once) * each
         else:
-            wanted = 4 * self.lib.skv_attention_kv4_scratch(min(n_seqs, KV4_SEQS), max_q_len, table_width, num_heads, num_kv_heads,
+            wanted = 4 * self.lib.skv_attention_kv4_scratch(at_once, max_q_len, table_width, num_heads, num_kv_heads,
                                                             block_size, window)
         if len(self._kv4_plans) > 4096:
             self._kv4_plans.clear()
-        self._kv4_plans[key] = (width, wanted, window)
-        return width, wanted, window
+        self._kv4_plans[key] = (width, wanted, window, at_once)
+        return width, wanted, window, at_once
 
     def attention_kv4_scratch(self, n_seqs: int, n_tokens: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int,
                               head_dim: int, block_size: int, window: int = 0) -> int:
@@ -1580,7 +1585,7 @@ class Kernels:
         """Causal attention over a cache held in 4 bits (bfloat16 build): sequence ``s`` owns rows ``cu_q[s]..cu_q[s+1]-1`` of
         ``q``/``out`` (at most ``max_q_len``), ``ctx_after[s]`` positions are cached, this step's included.  One or a few new tokens a sequence
         read the cache as it lies; many read the bfloat16 numbers it stands for (``unpack_kv4``, then
-        ``attention_prefill_tc``).  ``scratch``: uint8, at least ``attention_kv4_scratch`` bytes; two steps that may run at once need one each.
+        ``attention_prefill_tc``, by which a value's NaN reaches all queries of a tile, as over a 16-bit cache).  ``scratch``: uint8, at least ``attention_kv4_scratch`` bytes; two steps that may run at once need one each.
         A step's sums are cut by all its sequences' lengths, so that a sequence's result may differ in their order between batches."""
         u8, i32 = torch.uint8, torch.int32
         self._want_all("attention_kv4", (q, self.dtype, "q"), (out, self.dtype, "out"), (k_codes, u8, "k_codes"), (v_codes, u8, "v_codes"),
@@ -1592,27 +1597,29 @@ class Kernels:
             raise KernelError("attention_kv4: one length, one offset pair and one table row per sequence is needed")
         if q.shape != (n, num_heads * head_dim) or out.shape != q.shape or max_q_len < 1:
             raise KernelError("attention_kv4: q and out must be [tokens, heads * head_dim]")
-        width, wanted, window = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
+        width, wanted, window, at_once = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
         if wanted:
             if scratch is None or scratch.numel() < wanted:
                 raise KernelError(f"attention_kv4: {wanted} bytes of scratch are needed, not {0 if scratch is None else scratch.numel()}")
             self._want_all("attention_kv4", (scratch, u8, "scratch"))
         if width:
             # keys, values and their block table lie in the scratch one behind the other
-            blocks, keys = n_seqs * width, scratch.data_ptr()
-            values = keys + 2 * blocks * num_kv_heads * block_size * head_dim
-            table = values + 2 * blocks * num_kv_heads * block_size * head_dim
-            self._check(self.lib.skv_unpack_kv4(
-                k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), table_width,
-                ctx_after.data_ptr(), keys, values, table, n_seqs, width, num_kv_heads, head_dim, block_size,
-                window + max_q_len - 1 if window > 0 else 0, _stream()), "unpack_kv4")
-            pointer, zero = ctypes.c_void_p, ctypes.c_float(0.0)
-            self._check(self.lib.skv_attention_prefill_tc_extras(
-                _ptr(q), pointer(keys), pointer(values), blocks, pointer(table), table_width, _ptr(cu_q), _ptr(ctx_after), _ptr(out), n_seqs, n,
-                max_q_len, num_heads, num_kv_heads, head_dim, block_size, ctypes.c_float(scale), window, _NULL, 0, _NULL, 0, zero, 0, _NULL,
-                _ptr(flag if flag is not None else self.error_flag), _stream()), "attention_prefill_tc")
+            pointer, zero, keys = ctypes.c_void_p, ctypes.c_float(0.0), scratch.data_ptr()
+            for at in range(0, n_seqs, at_once):               # (int32 tensors: four bytes an entry)
+                seqs = min(n_seqs - at, at_once)
+                values = keys + 2 * seqs * width * num_kv_heads * block_size * head_dim
+                table = values + 2 * seqs * width * num_kv_heads * block_size * head_dim
+                lengths = ctx_after.data_ptr() + 4 * at
+                self._check(self.lib.skv_unpack_kv4(
+                    k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr() + 4 * at * table_width,
+                    table_width, lengths, keys, values, table, seqs, width, num_kv_heads, head_dim, block_size,
+                    window + max_q_len - 1 if window > 0 else 0, _stream()), "unpack_kv4")
+                self._check(self.lib.skv_attention_prefill_tc_extras(
+                    _ptr(q), pointer(keys), pointer(values), seqs * width, pointer(table), table_width, pointer(cu_q.data_ptr() + 4 * at),
+                    pointer(lengths), _ptr(out), seqs, n, max_q_len, num_heads, num_kv_heads, head_dim, block_size, ctypes.c_float(scale), window,
+                    _NULL, 0, _NULL, 0, zero, 0, _NULL, _ptr(flag if flag is not None else self.error_flag), _stream()), "attention_prefill_tc")
             return
-        for at in range(0, n_seqs, KV4_SEQS):                  # (int32 tensors: four bytes an entry)
+        for at in range(0, n_seqs, KV4_SEQS):
             self._check(self.lib.skv_attention_kv4(
                 q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                 block_table.data_ptr() + 4 * at * table_width, table_width, cu_q.data_ptr() + 4 * at, ctx_after.data_ptr() + 4 * at,

@@ -393,6 +393,32 @@ def test_lengths_that_contradict_the_call_spoil_no_other_sequence():
             torch.testing.assert_close(got[cu[s]].float(), alone[0].float(), rtol=2 * HALF_STEP, atol=twice_off(cache, False))
 
 
+@pytest.mark.parametrize("some", [1, 2])
+@pytest.mark.parametrize("window", [0, 150])
+def test_prompts_are_read_back_a_few_sequences_at_a_time(monkeypatch, some, window):
+    """The same results from a scratch that holds one sequence, or two, as from one that holds all."""
+    from stratakv_b200 import ops
+    k = lib(64)
+    heads, kv, block, before, new = 8, 2, 64, [900, 0, 40, 700, 3], [130, 200, 1, 65, 129]
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, 64, block, lengths)
+    cu = [0]
+    for c in new:
+        cu.append(cu[-1] + c)
+    q = torch.randn(cu[-1], heads * 64, device="cuda").bfloat16()
+    whole = k.attention_kv4_scratch(5, cu[-1], 200, table.shape[1], heads, kv, 64, block, window)
+    at_once = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
+    k._kv4_plans.clear()
+    monkeypatch.setattr(ops, "KV4_UNPACKED", whole // 5 * some)
+    try:
+        assert k.attention_kv4_scratch(5, cu[-1], 200, table.shape[1], heads, kv, 64, block, window) == whole // 5 * some
+        got = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
+    finally:
+        k._kv4_plans.clear()
+    # (blocks of the prompt kernel may share a tile's keys where there are few: sums in another order)
+    torch.testing.assert_close(got.float(), at_once.float(), rtol=2 * HALF_STEP, atol=twice_off(cache, True))
+
+
 @pytest.mark.parametrize("n_seqs,most", [(1100, 1), (2051, 2)])
 def test_more_sequences_than_a_launch_takes(n_seqs, most):
     k = lib(64)
