@@ -16,6 +16,7 @@
 
 #include "kv4.cuh"
 
+#include <array>
 #include <type_traits>
 
 #if SKV_DTYPE == SKV_BF16
@@ -122,15 +123,61 @@ __device__ __forceinline__ Kv4Share kv4_share(const Kv4Cut& cut, const int* cu_q
     return s;
 }
 
-template <int NT, int CK>
+// Bytes that the partial results of a block's warps take, and behind them those of the block.
+template <int NT> constexpr int ITEM_OF = (KV4_WARPS + 1) * NT * (OTILE4 * 512 + 64);
+template <int NT, int CK, bool ITEM> constexpr int KV4_SMEM = ITEM && ITEM_OF<NT> > RING_OF<CK> ? ITEM_OF<NT> : RING_OF<CK>;
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+// The same place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ float4 of_block(uint32_t at, int rank) {
+    float4 v;
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at), "r"(rank) : "memory");
+    return v;
+}
+
+// `parts` partial results of a tile of 16 numbers, brought to their common maximum and added up in their order.
+template <class Load>
+__device__ __forceinline__ void kv4_add_up(int parts, const Load& load, float4& acc, float4& ml) {
+    constexpr int AHEAD = 8;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    ml = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+    for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+        float4 o[AHEAD], of[AHEAD];                   // (maximum and sum of rows 2t and 2t + 1)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            of[u] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+            if (p0 + u < parts) load(p0 + u, o[u], of[u]);
+        }
+        float2 now = make_float2(ml.x, ml.z);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) now = make_float2(fmaxf(now.x, of[u].x), fmaxf(now.y, of[u].z));
+        const float2 by = make_float2(part_weight(ml.x, now.x), part_weight(ml.z, now.y));
+        acc = make_float4(acc.x * by.x, acc.y * by.y, acc.z * by.x, acc.w * by.y);
+        ml = make_float4(now.x, ml.y * by.x, now.y, ml.w * by.y);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const float a = part_weight(of[u].x, now.x), b = part_weight(of[u].z, now.y);
+            acc = make_float4(acc.x + o[u].x * a, acc.y + o[u].y * b, acc.z + o[u].z * a, acc.w + o[u].w * b);
+            ml.y += of[u].y * a;
+            ml.w += of[u].w * b;
+        }
+    }
+}
+
+// ITEM: a cluster of blocks has one item, whose chunks its warps share out and whose partial results it adds up itself.
+template <int NT, int CK, bool ITEM>
 __global__ void __launch_bounds__(KV4_WARPS * 32, NT == 1 && FHD <= 128 ? 2 : 1)
 kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes,
                      const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale, const int* __restrict__ block_table,
                      int table_width, const int* __restrict__ cu_q, const int* __restrict__ ctx_after, __nv_bfloat16* __restrict__ out,
                      float4* __restrict__ partial_o, float2* __restrict__ partial_ml, const Kv4Cut cut, int block_size, float scale,
-                     uint32_t chunks_magic, uint32_t ones) {
+                     uint32_t chunks_magic, uint32_t ones, int cluster) {
     extern __shared__ __align__(16) uint8_t kv4_smem[];
-    __shared__ int upto_all[KV4_SEQS], warp_all[KV4_WARPS];
+    __shared__ int upto_all[ITEM ? 1 : KV4_SEQS], warp_all[KV4_WARPS];
     constexpr int ROWS = 8 * NT;
     pdl_launch_dependents();
     pdl_wait();
@@ -140,7 +187,7 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     // upto[s]: the chunks up to and with sequence s.  Up to 32 sequences every warp adds up by itself, which needs no barrier.
     const bool few = cut.n_seqs <= 32;
     const int* upto = few ? upto_all + 32 * warp : upto_all;
-    for (int s0 = 0; s0 < cut.n_seqs; s0 += KV4_WARPS * 32) {
+    for (int s0 = 0; !ITEM && s0 < cut.n_seqs; s0 += KV4_WARPS * 32) {
         int sum = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, s0 + (few ? lane : (int)threadIdx.x)).all(cut);
 #pragma unroll
         for (int o2 = 1; o2 < 32; o2 *= 2) {
@@ -166,22 +213,29 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     const int workers = (int)gridDim.x * KV4_WARPS, run = max(cut.least, (total + workers - 1) / workers);
     const int worker = blockIdx.x + gridDim.x * warp;       // (runs that follow each other lie on different SMs)
     const long long run_begin = (long long)worker * run;
-    if (run_begin >= total) return;
-    const int run_end = (int)min((long long)total, run_begin + run);
+    if (!ITEM && run_begin >= total) return;
+    const int run_end = ITEM ? 1 : (int)min((long long)total, run_begin + run);
     int seq = 0;                                            // the first whose chunks reach beyond run_begin
-    for (int step = few ? 16 : KV4_SEQS / 2; step > 0; step /= 2)
+    for (int step = few ? 16 : KV4_SEQS / 2; !ITEM && step > 0; step /= 2)
         if (seq + step <= cut.n_seqs && upto[seq + step - 1] <= (int)run_begin) seq += step;
 
-    for (int done = (int)run_begin; done < run_end;) {
-    while (upto[seq] <= done) ++seq;                        // (sequences without tokens have no chunks)
+    for (int done = ITEM ? 0 : (int)run_begin; done < run_end;) {
+    const int of_cluster = ITEM ? blockIdx.x / cluster : 0, rank = blockIdx.x - of_cluster * cluster, items = num_kv_heads * cut.most_tiles;
+    if (ITEM) seq = of_cluster / items;
+    else
+        while (upto[seq] <= done) ++seq;                    // (sequences without tokens have no chunks)
     const Kv4Share share = kv4_share<ROWS, CK>(cut, cu_q, ctx_after, seq);
     const int q_begin = share.q_begin, q_len = share.q_len, tiles = share.tiles;
-    const int in_seq = done - (seq ? upto[seq - 1] : 0), item = in_seq / share.chunks, from = in_seq - item * share.chunks;
-    const int count = min(run_end - done, share.chunks - from), kv_head = item / tiles;
-    const bool whole = count == share.chunks;
+    const int in_seq = ITEM ? 0 : done - (seq ? upto[seq - 1] : 0), item = ITEM ? of_cluster - seq * items : in_seq / share.chunks;
+    const int kv_head = item / (ITEM ? cut.most_tiles : tiles), at_tile = item - kv_head * (ITEM ? cut.most_tiles : tiles);
+    // (ITEM: a tile behind the sequence's last has no chunks)
+    const int mine = ITEM && at_tile < tiles ? (share.chunks + cluster * KV4_WARPS - 1) / (cluster * KV4_WARPS) : 0;
+    const int from = ITEM ? (rank * KV4_WARPS + warp) * mine : in_seq - item * share.chunks;
+    const int count = ITEM ? max(0, min(mine, share.chunks - from)) : min(run_end - done, share.chunks - from);
+    const bool whole = !ITEM && count == share.chunks;
     const size_t slot = (size_t)2 * worker + (done != (int)run_begin);
-    done += count;
-    const int row0 = (item - kv_head * tiles) * ROWS, rows = q_len * group, before = share.ctx - q_len;
+    done += ITEM ? 1 : count;
+    const int row0 = at_tile * ROWS, rows = q_len * group, before = share.ctx - q_len;
     const int last_query = min(rows, row0 + ROWS) - 1;
     const int end = before + cut.of_group(last_query) + 1;                        // keys that any row of the tile sees lie before it
     const int my_first = share.first_chunk + from, my_end = min(my_first + count, (end + CK - 1) / CK);
@@ -514,12 +568,64 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
     ring_wait<0>();
     __syncwarp();                                     // (the next item's chunks go where these were)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int o2 = 4; o2 < 32; o2 *= 2) {
             sum[n].x += __shfl_xor_sync(0xffffffffu, sum[n].x, o2);
             sum[n].y += __shfl_xor_sync(0xffffffffu, sum[n].y, o2);
         }
+    if (ITEM) {
+        // Partial results as they lie in the registers, where the chunks were: a tile's 32 lanes of four numbers, then maxima and sums, a row each.
+        constexpr int TILES = NT * OTILE4, OF_WARP = NT * (OTILE4 * 512 + 64);
+        float4* parts_o = (float4*)kv4_smem;
+        float4* parts_ml = (float4*)(kv4_smem + (KV4_WARPS + 1) * TILES * 512);
+        static_assert(ITEM_OF<NT> == (KV4_WARPS + 1) * OF_WARP, "tiles, then maxima and sums");
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < OTILE4; ++j)
+                parts_o[(warp * TILES + n * OTILE4 + j) * 32 + lane] = make_float4(o[j][n][0], o[j][n][1], o[j][n][2], o[j][n][3]);
+            if (g == 0) parts_ml[(warp * NT + n) * 4 + t] = make_float4(-lift[n].x, sum[n].x, -lift[n].y, sum[n].y);
+        }
+        __syncthreads();
+        float4 acc[(TILES + KV4_WARPS - 1) / KV4_WARPS], ml[(TILES + KV4_WARPS - 1) / KV4_WARPS];
+#pragma unroll
+        for (int u = 0; u * KV4_WARPS < TILES; ++u) {
+            const int tile = u * KV4_WARPS + warp, n = tile / OTILE4;
+            if (tile >= TILES) continue;
+            kv4_add_up(KV4_WARPS, [&](int p, float4& v, float4& of) { v = parts_o[(p * TILES + tile) * 32 + lane]; of = parts_ml[(p * NT + n) * 4 + t]; }, acc[u], ml[u]);
+            if (cluster > 1) {
+                parts_o[(KV4_WARPS * TILES + tile) * 32 + lane] = acc[u];
+                if (g == 0 && tile % OTILE4 == 0) parts_ml[(KV4_WARPS * NT + n) * 4 + t] = ml[u];
+            }
+        }
+        if (cluster > 1) cluster_barrier();           // (every block of a cluster comes here, and to the one below)
+#pragma unroll
+        for (int u = 0; u * KV4_WARPS < TILES; ++u) {
+            const int tile = u * KV4_WARPS + warp, n = tile / OTILE4, j = tile - n * OTILE4;
+            if (tile >= TILES || tile % cluster != rank) continue;
+            if (cluster > 1)
+                kv4_add_up(cluster, [&](int p, float4& v, float4& of) {
+                    v = of_block(smem_u32(parts_o + (KV4_WARPS * TILES + tile) * 32 + lane), p);
+                    of = of_block(smem_u32(parts_ml + (KV4_WARPS * NT + n) * 4 + t), p);
+                }, acc[u], ml[u]);
+            const int d = g * (FPAD / 8) + 2 * j;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int r = row0 + 8 * n + 2 * t + c;
+                if (r >= rows || d >= FHD || share.chunks == 0) continue;
+                const int token = cut.of_group(r);
+                const float by = 1.0f / (c ? ml[u].w : ml[u].y);
+                *(__nv_bfloat162*)(out + ((size_t)(q_begin + token) * num_heads + kv_head * group + r - token * group) * FHD + d) =
+                    __floats2bfloat162_rn((c ? acc[u].y : acc[u].x) * by, (c ? acc[u].w : acc[u].z) * by);
+            }
+        }
+        if (cluster > 1) cluster_barrier();           // (a block's shared memory lasts until all have read it)
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
         if (!whole) {
             // left as they lie in the registers: a lane's four numbers of a tile
 #pragma unroll
@@ -555,7 +661,7 @@ template <int NT, int CK, bool SPREAD>
 __global__ void __launch_bounds__(KV4_WARPS * 32)
 kv4_merge_kernel(const float4* __restrict__ partial_o, const float4* __restrict__ partial_ml, const int* __restrict__ cu_q,
                  const int* __restrict__ ctx_after, __nv_bfloat16* __restrict__ out, const Kv4Cut cut, int workers) {
-    constexpr int ROWS = 8 * NT, AHEAD = 8;
+    constexpr int ROWS = 8 * NT;
     __shared__ float4 shared_o[KV4_WARPS][32], shared_ml[KV4_WARPS][32];
     __shared__ int sums[2][KV4_WARPS];
     pdl_launch_dependents();
@@ -584,45 +690,19 @@ kv4_merge_kernel(const float4* __restrict__ partial_o, const float4* __restrict_
     auto slot_of = [&](int p) { return (size_t)2 * (first + p) + (p == 0 && begin != first * run); };
     for (int tile = SPREAD ? blockIdx.y : blockIdx.y * KV4_WARPS + warp; tile < OTILE4 * NT; tile += SPREAD ? OTILE4 * NT : KV4_WARPS * (int)gridDim.y) {
         const int n = tile / OTILE4, j = tile - n * OTILE4;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float2 top = make_float2(-INFINITY, -INFINITY), sum = make_float2(0.0f, 0.0f);
-        for (int p0 = SPREAD ? warp : 0; p0 < parts; p0 += AHEAD * (SPREAD ? KV4_WARPS : 1)) {
-            float4 o[AHEAD], ml[AHEAD];               // (maximum and sum of rows 2t and 2t + 1)
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int p = p0 + u * (SPREAD ? KV4_WARPS : 1);
-                const size_t at = slot_of(p);
-                o[u] = p < parts ? partial_o[((at * NT + n) * OTILE4 + j) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                ml[u] = p < parts ? partial_ml[at * (ROWS / 2) + 4 * n + t] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-            }
-            float2 now = top;
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) now = make_float2(fmaxf(now.x, ml[u].x), fmaxf(now.y, ml[u].z));
-            const float2 by = make_float2(part_weight(top.x, now.x), part_weight(top.y, now.y));
-            acc = make_float4(acc.x * by.x, acc.y * by.y, acc.z * by.x, acc.w * by.y);
-            sum = make_float2(sum.x * by.x, sum.y * by.y);
-            top = now;
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const float a = part_weight(ml[u].x, now.x), b = part_weight(ml[u].z, now.y);
-                acc = make_float4(acc.x + o[u].x * a, acc.y + o[u].y * b, acc.z + o[u].z * a, acc.w + o[u].w * b);
-                sum = make_float2(sum.x + ml[u].y * a, sum.y + ml[u].w * b);
-            }
-        }
+        float4 acc, ml;
+        const int own = SPREAD ? warp : 0, step = SPREAD ? KV4_WARPS : 1;
+        kv4_add_up((parts - own + step - 1) / step, [&](int p, float4& v, float4& of) {
+            const size_t at = slot_of(own + p * step);
+            v = partial_o[((at * NT + n) * OTILE4 + j) * 32 + lane];
+            of = partial_ml[at * (ROWS / 2) + 4 * n + t];
+        }, acc, ml);
         if (SPREAD) {
             shared_o[warp][lane] = acc;
-            shared_ml[warp][lane] = make_float4(top.x, sum.x, top.y, sum.y);
+            shared_ml[warp][lane] = ml;
             __syncthreads();
             if (warp != 0) return;
-            acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            sum = make_float2(0.0f, 0.0f);
-            for (int w = 0; w < KV4_WARPS; ++w) top = make_float2(fmaxf(top.x, shared_ml[w][lane].x), fmaxf(top.y, shared_ml[w][lane].z));
-            for (int w = 0; w < KV4_WARPS; ++w) {
-                const float4 v = shared_o[w][lane], ml = shared_ml[w][lane];
-                const float a = part_weight(ml.x, top.x), b = part_weight(ml.z, top.y);
-                acc = make_float4(acc.x + v.x * a, acc.y + v.y * b, acc.z + v.z * a, acc.w + v.w * b);
-                sum = make_float2(sum.x + ml.y * a, sum.y + ml.w * b);
-            }
+            kv4_add_up(KV4_WARPS, [&](int p, float4& v, float4& of) { v = shared_o[p][lane]; of = shared_ml[p][lane]; }, acc, ml);
         }
         const int d = g * (FPAD / 8) + 2 * j;
         if (d >= FHD) continue;
@@ -631,17 +711,45 @@ kv4_merge_kernel(const float4* __restrict__ partial_o, const float4* __restrict_
             const int r = at_tile * ROWS + 8 * n + 2 * t + c;
             if (r >= share.q_len * group) continue;
             const int token = cut.of_group(r);
-            const float by = 1.0f / (c ? sum.y : sum.x);
+            const float by = 1.0f / (c ? ml.w : ml.y);
             *(__nv_bfloat162*)(out + ((size_t)(share.q_begin + token) * cut.num_heads + kv_head * group + r - token * group) * FHD + d) =
                 __floats2bfloat162_rn((c ? acc.y : acc.x) * by, (c ? acc.w : acc.z) * by);
         }
     }
 }
 
+// Clusters of `size` blocks that fit the GPU at once, by variant of the kernel (0 where there is no GPU).
+template <int NT, int CK>
+static int fitting_clusters(int size) {
+    if (reserve_shared_once<kv4_attention_kernel<NT, CK, true>>("skv_attention_kv4", KV4_SMEM<NT, CK, true>)) return 0;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(size);
+    config.blockDim = dim3(KV4_WARPS * 32);
+    config.dynamicSmemBytes = KV4_SMEM<NT, CK, true>;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = size;
+    attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    int count = 0;
+    return cudaOccupancyMaxActiveClusters(&count, kv4_attention_kernel<NT, CK, true>, &config) == cudaSuccess ? count : 0;
+}
+static int most_clusters(int variant, int size) {
+    static const std::array<std::array<int, 4>, 4> fit = [] {
+        std::array<std::array<int, 4>, 4> of;
+        for (int i = 0; i < 4; ++i)
+            of[0][i] = fitting_clusters<1, 32>(1 << i), of[1][i] = fitting_clusters<1, 16>(1 << i), of[2][i] = fitting_clusters<2, 32>(1 << i),
+            of[3][i] = fitting_clusters<2, 16>(1 << i);
+        return of;
+    }();
+    return fit[variant][size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3];
+}
+
 // How a step of these sizes is cut: as many runs as warps fit the GPU, and how many partial results an item has at most.
 struct Kv4Plan {
     Kv4Cut cut;
-    int chunk, tiles_of_8, blocks;
+    int chunk, tiles_of_8, blocks, cluster;           // (cluster: blocks of an item, 0 where runs are dealt out)
     long long items, chunks, parts, floats;
 };
 
@@ -664,8 +772,21 @@ static Kv4Plan kv4_plan(int n_seqs, int max_q_len, int table_width, int num_head
     const long long workers = (long long)plan.blocks * KV4_WARPS, run = plan.chunks / workers > least ? plan.chunks / workers : least;
     const uint32_t group = (uint32_t)(num_heads / num_kv_heads);
     plan.cut = {n_seqs, num_heads, num_kv_heads, window, least, (int)most, max_q_len, row_tiles, (int)group, (uint32_t)((0x100000000ull + group - 1) / group)};
+    // Runs, or clusters?  Counted in rounds, a chunk for every warp: a cluster's warps take as many as the longest item has chunks for them, and again
+    // for every wave of clusters that the GPU takes at once; runs take the mean, but their partial results pass through memory to a second launch.
+    // us, runs / clusters, heads of 128: 1 x 300 positions, 8 key heads (1 round / 1) 7.6 / 5.8; 1 x 8,000 (1 / 4) 12.3 / 10.0, 1 x 16,000 (2 / 8) 14.4 /
+    // 15.5; 8 x 4,000 (4 / 4) 19.6 / 14.0; 64 x 300 (3 / 2 waves of 2) 18.3 / 13.6; 32 key heads 64 x 1,000 (28 / 7 waves of 4) 85 / 79, 64 x 150 (5 / 7 waves
+    // of 1) 23.5 / 33.9.  Of ragged sequences a cluster waits for the longest: lengths that fall evenly from the longest to nothing 8 x 2,000, 32 key
+    // heads (8 rounds) 19.4 / 19.8, 8 x 4,000 (16 rounds) 28.7 / 35.5, all as long as the longest 24.7 / 20.5 and 41.0 / 37.4; so at most 8 rounds.
+    const int variant = 2 * (plan.tiles_of_8 - 1) + (plan.chunk == 16);
+    plan.cluster = 1;
+    while (plan.cluster < 8 && chunks > KV4_WARPS * plan.cluster && plan.items <= most_clusters(variant, 2 * plan.cluster)) plan.cluster *= 2;
+    const long long rounds = (chunks + KV4_WARPS * plan.cluster - 1) / (KV4_WARPS * plan.cluster), at_once = most_clusters(variant, plan.cluster);
+    const long long waves = at_once > 0 ? (plan.items + at_once - 1) / at_once : 1 << 30;
+    const long long of_runs = (plan.chunks + workers - 1) / workers;
+    if ((n_seqs > 1 && rounds > 8) || (waves == 1 ? rounds > of_runs + 3 : 4 * waves * (rounds + 1) > 5 * of_runs + 20)) plan.cluster = 0;
     plan.parts = chunks > 1 ? (chunks + run - 1) / run + 1 : 1;
-    plan.floats = plan.parts > 1 ? 2 * workers * 8 * plan.tiles_of_8 * (FPAD + 2) : 0;
+    plan.floats = plan.parts > 1 && !plan.cluster ? 2 * workers * 8 * plan.tiles_of_8 * (FPAD + 2) : 0;
     return plan;
 }
 
@@ -675,14 +796,34 @@ static int kv4_launch(const Kv4Plan& plan, const void* q, const void* k_codes, c
                       float scale, cudaStream_t stream) {
     // a chunk's block is chunk / (block_size / CK): the upper half of a product, exact while chunks x chunks a block stay below 2^32
     const uint32_t chunks_magic = block_size == CK ? 0u : (uint32_t)((0x100000000ull + block_size / CK - 1) / (block_size / CK));
-    if (int code = reserve_shared_once<kv4_attention_kernel<NT, CK>>("skv_attention_kv4", RING_OF<CK>)) return code;
     const int workers = plan.blocks * KV4_WARPS;
     float* partial_ml = plan.floats ? scratch + (size_t)2 * workers * 8 * NT * FPAD : nullptr;
-    if (int code = launch_pdl("skv_attention_kv4", kv4_attention_kernel<NT, CK>, dim3(plan.blocks), dim3(KV4_WARPS * 32), RING_OF<CK>, stream,
-                              (const __nv_bfloat16*)q, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale,
-                              block_table, table_width, cu_q, ctx_after, (__nv_bfloat16*)out, (float4*)scratch, (float2*)partial_ml, plan.cut, block_size,
-                              scale, chunks_magic, KV4_ONES))
-        return code;
+    auto start = [&](auto kernel, unsigned blocks, int smem) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(blocks);
+        config.blockDim = dim3(KV4_WARPS * 32);
+        config.dynamicSmemBytes = smem;
+        config.stream = stream;
+        cudaLaunchAttribute attributes[2];
+        attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+        attributes[1].id = cudaLaunchAttributeClusterDimension;
+        attributes[1].val.clusterDim.x = plan.cluster > 1 ? plan.cluster : 1;
+        attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+        config.attrs = attributes;
+        config.numAttrs = plan.cluster > 1 ? 2 : 1;
+        const cudaError_t status = cudaLaunchKernelEx(&config, kernel, (const __nv_bfloat16*)q, (const uint8_t*)k_codes, (const uint8_t*)v_codes,
+                                                      (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table, table_width, cu_q, ctx_after,
+                                                      (__nv_bfloat16*)out, (float4*)scratch, (float2*)partial_ml, plan.cut, block_size, scale,
+                                                      chunks_magic, KV4_ONES, plan.cluster);
+        return status == cudaSuccess ? 0 : fail("skv_attention_kv4", cudaGetErrorString(status));
+    };
+    if (plan.cluster) {
+        if (int code = reserve_shared_once<kv4_attention_kernel<NT, CK, true>>("skv_attention_kv4", KV4_SMEM<NT, CK, true>)) return code;
+        return start(kv4_attention_kernel<NT, CK, true>, (unsigned)(plan.items * plan.cluster), KV4_SMEM<NT, CK, true>);
+    }
+    if (int code = reserve_shared_once<kv4_attention_kernel<NT, CK, false>>("skv_attention_kv4", RING_OF<CK>)) return code;
+    if (int code = start(kv4_attention_kernel<NT, CK, false>, plan.blocks, RING_OF<CK>)) return code;
     if (plan.floats == 0) return 0;
     const bool spread = plan.parts > 9 && plan.items * OTILE4 * NT <= 2 * sm_count();
     auto merge = spread ? kv4_merge_kernel<NT, CK, true> : kv4_merge_kernel<NT, CK, false>;

@@ -1466,6 +1466,7 @@ class Kernels:
         self.lib.skv_attention_kv4_scratch.argtypes = [i] * 7
         self.lib.skv_attention_kv4_scratch.restype = ctypes.c_longlong
         self._kv4_plans = {}
+        self._kv4_sms = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
         self._kv4_prototyped = True
 
     def _want_all(self, call: str, *wanted) -> None:
@@ -1534,33 +1535,40 @@ class Kernels:
             head_dim, block_size, int(keep), _stream()), "unpack_kv4")
 
     @staticmethod
-    def _kv4_few(max_q_len: int, group: int, positions: int) -> bool:
+    def _kv4_few(n_seqs: int, max_q_len: int, group: int, num_kv_heads: int, positions: int, sms: int) -> bool:
         """Whether ``attention_kv4`` reads the 4-bit cache itself.  It then unpacks a key head's codes again for every 16 rows (``group`` query
         heads of each new token), while unpacking them once for the tensor-core prompt kernel costs that kernel's whole tile of 128 queries for
-        every query head: 8 sequences of 8,000 positions, heads of 128, us, by rows of a key head: 32 heads over 8, 128 rows 168 / 241, 192 rows
-        247 / 241; 32 over 32, 48 rows 248 / 510; 32 heads of 64 over 4, 256 rows 111 / 152, 384 rows 163 / 150.  So the rows at which both take as
-        long grow with the group: 16 (2 group + 4).  Over a few hundred positions both are a chain of latencies, the prompt kernel's the shorter
-        (300 positions, 32 heads over 8 of 128: 32 rows 10.6 / 11.3, 64 rows 13.6 / 11.4)."""
-        return max_q_len * group <= (16 * (2 * group + 4) if positions > 512 else 48)
+        every query head: 8 sequences of 8,000 positions, heads of 128, us, by rows of a key head: 32 heads over 8, 128 rows 165 / 239, 192 rows
+        242 / 240; 32 over 32, 48 rows 243 / 506; 32 heads of 64 over 4, 256 rows 107 / 149, 384 rows 157 / 149.  So the rows at which both take as
+        long grow with the group: 16 (2 group + 4), and over a few hundred positions, where either is a chain of latencies, it is 48.  Tiles of 16 rows
+        that the GPU takes at once are served sooner than two launches whatever the group: 1 sequence, 32 heads of 64 over 4, 512 rows over 300 / 1,000 /
+        4,000 positions 5.4 / 10.3, 7.2 / 17.5, 18.0 / 24.4; 32 heads of 128 over 8, two waves of them, 4 of 1,000 20.5 / 26.3, 8 of 300 14.7 / 17.1."""
+        rows, tiles = max_q_len * group, n_seqs * num_kv_heads * -(-max_q_len * group // 16)
+        return rows <= (16 * (2 * group + 4) if positions > 512 else 48) or (positions <= 4096 and tiles <= (2 if positions > 256 else 1) * sms)
 
-    def _kv4_plan(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+    def _kv4_plan(self, *sizes) -> Tuple[int, int, int, int]:
+        """``_kv4_plan_of`` these sizes, kept."""
+        if not self._kv4_prototyped:
+            self._kv4_prototypes()
+        plan = self._kv4_plans.get(sizes)
+        if plan is None:
+            if len(self._kv4_plans) > 4096:
+                self._kv4_plans.clear()
+            plan = self._kv4_plans[sizes] = self._kv4_plan_of(*sizes)
+        return plan
+
+    def _kv4_plan_of(self, n_seqs: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
                   window: int) -> Tuple[int, int, int, int]:
         """How ``attention_kv4`` serves a step of these sizes: (blocks of each sequence that it reads through ``unpack_kv4``, 0
         where it reads the 4-bit cache itself; bytes of scratch; the window, 0 for one that the table's positions cannot leave;
         sequences that it takes at once)."""
-        if not self._kv4_prototyped:
-            self._kv4_prototypes()
-        key = (n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
-        plan = self._kv4_plans.get(key)
-        if plan is not None:
-            return plan
         if window < 0:
             raise KernelError("attention_kv4: a window must not be negative")
         if window >= table_width * block_size:
             window = 0
         width, at_once, tiles = 0, min(n_seqs, KV4_SEQS), -(-max_q_len // 128)
-        if (not self._kv4_few(max_q_len, num_heads // max(1, num_kv_heads), table_width * block_size) and block_size & (block_size - 1) == 0 and block_size >= 16
-                and self.has_attention_prefill_tc() and head_dim == self.head_dim and tiles <= 65535):
+        if (not self._kv4_few(n_seqs, max_q_len, num_heads // max(1, num_kv_heads), num_kv_heads, table_width * block_size, self._kv4_sms)
+                and block_size & (block_size - 1) == 0 and block_size >= 16 and self.has_attention_prefill_tc() and head_dim == self.head_dim and tiles <= 65535):
             width = table_width if window == 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
         if width:
             # every sequence has room for the longest: a long one among many short ones must not ask for many times the cache
@@ -1570,9 +1578,6 @@ class Kernels:
         else:
             wanted = 4 * self.lib.skv_attention_kv4_scratch(at_once, max_q_len, table_width, num_heads, num_kv_heads,
                                                             block_size, window)
-        if len(self._kv4_plans) > 4096:
-            self._kv4_plans.clear()
-        self._kv4_plans[key] = (width, wanted, window, at_once)
         return width, wanted, window, at_once
 
     def attention_kv4_scratch(self, n_seqs: int, n_tokens: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int,

@@ -151,6 +151,13 @@ def test_unpack_gives_what_the_codes_stand_for(kv, dim, block, lengths, keep, wi
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
 
+def take(monkeypatch, few):
+    """Whether steps read the 4-bit cache themselves or what unpack_kv4 gives."""
+    from stratakv_b200.ops import Kernels
+    monkeypatch.setattr(Kernels, "_kv4_few", staticmethod(lambda *sizes: few))
+    monkeypatch.setattr(Kernels, "_kv4_plan", lambda self, *sizes: (self._kv4_prototyped or self._kv4_prototypes()) and None or self._kv4_plan_of(*sizes))
+
+
 def check_attention(heads, kv, dim, block, before, new, window=0, spread=1.0, extra_rows=0, table_room=0):
     k = lib(dim)
     lengths = [b + n for b, n in zip(before, new)]
@@ -202,12 +209,35 @@ def test_attention_of_a_few_tokens_a_sequence(heads, kv, dim, block, before, new
     (4, 2, 64, 64, [0], [300], 0), (4, 1, 128, 16, [77, 0, 900], [130, 1, 40], 0), (8, 8, 64, 32, [1000, 5], [65, 200], 100),
     (2, 1, 128, 128, [3], [513], 64), (8, 2, 64, 64, [0] * 5, [100, 1, 64, 65, 33], 0), (4, 4, 128, 64, [700, 0], [97, 96], 0),
     (8, 1, 64, 16, [600], [41], 0)])
-def test_attention_of_prompts(heads, kv, dim, block, before, new, window):
+@pytest.mark.parametrize("few", [False, True])
+def test_attention_of_prompts(monkeypatch, heads, kv, dim, block, before, new, window, few):
+    """Both ways, whichever the rule would take."""
+    take(monkeypatch, few)
     check_attention(heads, kv, dim, block, before, new, window)
 
 
+# (sequences so long that runs of chunks are dealt out, whose partial results a second launch adds up)
+@pytest.mark.parametrize("heads,kv,dim,block,before,new,window", [
+    (4, 2, 16, 16, [9000, 70], [1, 1], 0), (8, 1, 48, 64, [17000, 3], [1, 1], 0), (32, 4, 64, 64, [17000, 511], [1, 1], 0), (3, 3, 80, 16, [9000, 0], [6, 2], 0),
+    (16, 2, 128, 64, [17000, 40], [1, 3], 0), (8, 8, 128, 16, [40, 9000], [1, 1], 0), (2, 1, 208, 16, [9000, 1], [1, 1], 0), (4, 1, 256, 64, [18000, 50], [1, 1], 17000),
+    (24, 1, 64, 16, [9000, 17], [1, 2], 8500), (6, 2, 192, 64, [1, 17000], [1, 4], 0), (32, 8, 128, 64, [40000], [1], 0), (4, 4, 64, 64, [100_000], [1], 0)])
+def test_attention_by_runs(heads, kv, dim, block, before, new, window):
+    width = -(-max(b + n for b, n in zip(before, new)) // block)
+    assert lib(dim).attention_kv4_scratch(len(new), sum(new), max(new), width, heads, kv, dim, block, window) > 0
+    check_attention(heads, kv, dim, block, before, new, window)
+
+
+def test_a_cluster_for_every_item_needs_no_scratch():
+    """One block, a few, several waves of single ones."""
+    for sizes in ((1, 1, 1, 4, 2, 64, 16), (1, 1, 30, 4, 2, 64, 64), (8, 1, 60, 32, 8, 64, 64), (100, 1, 5, 32, 4, 64, 64), (3, 9, 20, 8, 2, 64, 32)):
+        assert lib(64).attention_kv4_scratch(sizes[0], sizes[0] * sizes[1], *sizes[1:]) == 0
+    check_attention(32, 4, 64, 64, [290 + i % 30 for i in range(100)], [1] * 100)
+    check_attention(8, 8, 128, 16, [(37 * i) % 150 for i in range(64)], [1 + i % 2 for i in range(64)])
+
+
 @pytest.mark.parametrize("new", [[1, 1], [4, 2], [100, 30]])
-def test_attention_leaves_rows_behind_the_last_sequence(new):
+def test_attention_leaves_rows_behind_the_last_sequence(monkeypatch, new):
+    take(monkeypatch, new[0] < 100)
     check_attention(4, 2, 64, 32, [3000, 600], new, extra_rows=5, table_room=3)
 
 
@@ -274,12 +304,13 @@ def twice_off(cache, unpacked):
 
 
 @pytest.mark.parametrize("new", [1, 4, 200])
-def test_windows_of_any_size(new):
+def test_windows_of_any_size(monkeypatch, new):
     """One as long as what is cached, or longer, changes nothing; a negative one is refused, whichever way the step takes."""
     from stratakv_b200.ops import KernelError
     k = lib(64)
     cache, table = make_cache(2, 64, 16, [300 + new])
     q = torch.randn(new, 4 * 64, device="cuda").bfloat16()
+    take(monkeypatch, new < 200)
     plain = run_step(k, q, cache, table, [0, new], [300 + new], 4, 2, 64, 16, new)
     for window in (300 + new, 10 ** 6, 2 ** 31 - new, 2 ** 31 - 1, 2 ** 32 + 5):
         got = run_step(k, q, cache, table, [0, new], [300 + new], 4, 2, 64, 16, new, window=window)
@@ -354,13 +385,14 @@ def test_append_read_back_and_attend_together():
         before = after
 
 
-def test_cases_here_reach_both_ways_of_attending():
-    """The rule that the parametrised cases above go by: a few tokens read the cache itself, prompts the numbers it stands for."""
+def test_which_way_a_step_attends():
+    """The rule: a few tokens read the cache itself, prompts the numbers it stands for."""
     k = lib(64)
-    assert k._kv4_plan(1, 1, 100, 4, 2, 64, 64, 0)[0] == 0 and k._kv4_plan(1, 300, 5, 4, 2, 64, 64, 0)[0] == 5
-    assert k._kv4_plan(2, 200, 20, 8, 8, 64, 64, 100)[0] == min(20, (100 + 200 - 1 + 62) // 64 + 1)
-    assert k._kv4_plan(1, 300, 5, 4, 2, 64, 48, 0)[0] == 0                 # (the prompt kernel wants blocks that are powers of two)
-    assert lib(80)._kv4_plan(1, 300, 5, 4, 2, 80, 64, 0)[0] == 0           # (and heads of 64 or 128)
+    assert k._kv4_plan(1, 1, 100, 4, 2, 64, 64, 0)[0] == 0 and k._kv4_plan(1, 2000, 40, 4, 2, 64, 64, 0)[0] == 40
+    assert k._kv4_plan(2, 900, 20, 8, 8, 64, 64, 100)[0] == min(20, (100 + 900 - 1 + 62) // 64 + 1)
+    assert k._kv4_plan(1, 300, 5, 4, 2, 64, 64, 0)[0] == 0 and k._kv4_plan(8, 300, 5, 4, 2, 64, 64, 0)[0] == 5     # (tiles for the whole GPU)
+    assert k._kv4_plan(1, 2000, 40, 4, 2, 64, 48, 0)[0] == 0               # (the prompt kernel wants blocks that are powers of two)
+    assert lib(80)._kv4_plan(1, 2000, 40, 4, 2, 80, 64, 0)[0] == 0         # (and heads of 64 or 128)
 
 
 @pytest.mark.parametrize("new", [[0, 1, 0, 1], [3, 0, 0, 2]])
@@ -406,15 +438,12 @@ def test_prompts_are_read_back_a_few_sequences_at_a_time(monkeypatch, some, wind
     for c in new:
         cu.append(cu[-1] + c)
     q = torch.randn(cu[-1], heads * 64, device="cuda").bfloat16()
+    take(monkeypatch, False)
     whole = k.attention_kv4_scratch(5, cu[-1], 200, table.shape[1], heads, kv, 64, block, window)
     at_once = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
-    k._kv4_plans.clear()
     monkeypatch.setattr(ops, "KV4_UNPACKED", whole // 5 * some)
-    try:
-        assert k.attention_kv4_scratch(5, cu[-1], 200, table.shape[1], heads, kv, 64, block, window) == whole // 5 * some
-        got = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
-    finally:
-        k._kv4_plans.clear()
+    assert k.attention_kv4_scratch(5, cu[-1], 200, table.shape[1], heads, kv, 64, block, window) == whole // 5 * some
+    got = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
     # (blocks of the prompt kernel may share a tile's keys where there are few: sums in another order)
     torch.testing.assert_close(got.float(), at_once.float(), rtol=2 * HALF_STEP, atol=twice_off(cache, True))
 
@@ -508,12 +537,10 @@ def test_refusals():
                           ("must be contiguous", dict(block_table=torch.cat([table, table], dim=1)[:, ::2])), ("CUDA tensor", dict(q=q.cpu()))):
         with pytest.raises(KernelError, match=match):
             attend(**change)
-    long_cache, long_table = make_cache(2, 64, 16, [4000])
-    with pytest.raises(KernelError, match="bytes of scratch are needed"):
-        attend(k_codes=long_cache[0], v_codes=long_cache[1], k_scale=long_cache[2], v_scale=long_cache[3], block_table=long_table, ctx_after=ints([4000]),
-               scratch=torch.empty(8, dtype=torch.uint8, device="cuda"))
-    with pytest.raises(KernelError, match="bytes of scratch are needed"):
-        attend(scratch=None)
+    long_table = torch.zeros(1, 2000, dtype=torch.int32, device="cuda")     # (sizes alone decide: this table could hold 32,000 positions)
+    for scratch in (torch.empty(8, dtype=torch.uint8, device="cuda"), None):
+        with pytest.raises(KernelError, match="bytes of scratch are needed"):
+            attend(block_table=long_table, scratch=scratch)
     qkv = torch.zeros(1, 8 * 64, device="cuda")
     with pytest.raises(KernelError, match="width does not match"):
         k.append_kv4(qkv[:, :256].contiguous(), None, ints([0]), ints([0]), table, out, *cache, 4, 2, 64, 16)
