@@ -779,8 +779,12 @@ static Kv4Plan kv4_plan(int n_seqs, int max_q_len, int table_width, int num_head
     // of 1) 23.5 / 33.9.  Of ragged sequences a cluster waits for the longest: lengths that fall evenly from the longest to nothing 8 x 2,000, 32 key
     // heads (8 rounds) 19.4 / 19.8, 8 x 4,000 (16 rounds) 28.7 / 35.5, all as long as the longest 24.7 / 20.5 and 41.0 / 37.4; so at most 8 rounds.
     const int variant = 2 * (plan.tiles_of_8 - 1) + (plan.chunk == 16);
+    // How many blocks: twice as many where each warp has more than one and a half chunks to lose (1 x 300 positions, 8 key heads of 128, one block 5.5, two
+    // 5.8; 8 x 1,000, two 9.7, four 8.1), as long as they fit.  Where clusters of eight just fill the GPU a model's step gains or loses a little against four,
+    // as its other kernels leave them room: a layer, 8 x 2,200, 4 key heads of 64 36.8 / 34.6; 4 x 2,200, 8 of 128 38.6 / 39.6; 1 x 3,000, 32 of 128
+    // 40.5 / 42.0 (runs 36.9, 41.8, 44.2).
     plan.cluster = 1;
-    while (plan.cluster < 8 && chunks > KV4_WARPS * plan.cluster && plan.items <= most_clusters(variant, 2 * plan.cluster)) plan.cluster *= 2;
+    while (plan.cluster < 8 && 2 * chunks > 3 * KV4_WARPS * plan.cluster && plan.items <= most_clusters(variant, 2 * plan.cluster)) plan.cluster *= 2;
     const long long rounds = (chunks + KV4_WARPS * plan.cluster - 1) / (KV4_WARPS * plan.cluster), at_once = most_clusters(variant, plan.cluster);
     const long long waves = at_once > 0 ? (plan.items + at_once - 1) / at_once : 1 << 30;
     const long long of_runs = (plan.chunks + workers - 1) / workers;
