@@ -5,13 +5,21 @@
 // in which what the cache holds is exact: a query is brought to a largest magnitude between 1 and 2 by a power of two (its 8
 // bits fit a half's 11), and the probabilities keep 11 bits.
 //
-// A block has up to 8 NT rows (a row: a query head of one new token; the heads that share a key head lie side by side), a warp 16 keys
-// at a time.  Both products are turned so that the keys are the rows of mma.sync m16n8k16: S^T = K Q^T, O^T = V^T P^T.  Eight rows
+// An item is a key head of a sequence and up to 8 NT rows (a row: a query head of one new token; the heads that share a key head lie side by side); a warp
+// takes 32 keys of it at a time (16 where a cache block is no multiple of 32), which asynchronous copies have brought to its own part of shared memory.
+// Both products are turned so that the keys are the rows of mma.sync m16n8k16: S^T = K Q^T, O^T = V^T P^T.  Eight rows
 // then fill an instruction, and a lane has eight keys' or values' numbers for each instead of four.  Which number of
 // a head is which index of the sum is free as long as both operands agree: lane t of four has a quarter of a key's numbers, one after
 // the other, so it reads its codes in one piece and one scale byte serves sixteen of them.  For the second product a lane has
 // a run of numbers of four keys; the bytes of two keys are put side by side ahead of the unpacking, which then yields the pairs of keys
 // that the instruction wants.  P goes from one product to the other by movmatrix.
+//
+// Over many positions it is bound by issue: a chunk of 32 keys of a head of 128 is 688 instructions of a warp, 352 of them unpacking (11 for eight codes),
+// and takes 1,000 cycles of a scheduler.  64 sequences of 4,096 positions, 32 heads over 8 of 128, 73 us, 4.1 TB/s of codes and scales; copies alone
+// 58, all but the copies 60.  (Loads by each lane 130 us; copies through shared memory, 16 keys at a time 101; 32 keys, packed float arithmetic, masks only
+// where a row needs them 83; one logic operation a code 74.  16 warps an SM at 128 registers: 18 to 20 spill, 97 to 106.)  On tcgen05 the unpacked codes
+// would go through shared memory first; the products here are a quarter of the time at most.
+// Over few positions it is a chain of latencies: lengths, block table, one or two chunks, and the sum over the warps.
 #include "head_size.cuh"
 
 #include "kv4.cuh"
@@ -94,8 +102,9 @@ constexpr float KV4_MARGIN = 8.0f, KV4_LIFT = 7.0f;
 // NaN was among them, which must not get lost.
 __device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY ? 1.0f : kv4_exp2(m - top); }
 
-// How a step's work is cut.  An item is one key head of a sequence for one tile of rows; the chunks of all items, one item behind the other, are dealt
-// out to the warps in runs of equal length.  A run that begins or ends inside an item leaves a partial result, at most two a warp; an item that
+// How a step's work is cut, in one of two ways (kv4_plan has the rule).  Either a cluster of one to eight blocks has an item and adds its warps' results
+// up in shared memory: one launch.  Or the chunks of all items, one item behind the other, are dealt
+// out to the warps in runs of equal length, whatever the sequences' lengths.  A run that begins or ends inside an item leaves a partial result, at most two a warp; an item that
 // one run holds whole is finished by it.  (Runs of blocks, whose warps take chunks in turn and add up in shared memory: 64 x 4,096 positions 79.6 us
 // against 73.9, 12 ragged sequences of 32 key heads 52.4 against 46.4.)
 struct Kv4Cut {
