@@ -1576,8 +1576,9 @@ class Kernels:
             at_once = max(1, min(n_seqs, KV4_UNPACKED // each, 65535 // tiles))
             wanted = min(n_seqs, at_once) * each
         else:
-            wanted = 4 * self.lib.skv_attention_kv4_scratch(at_once, max_q_len, table_width, num_heads, num_kv_heads,
-                                                            block_size, window)
+            # (the last launch's sequences may be cut in another way than a full one's)
+            wanted = 4 * max(self.lib.skv_attention_kv4_scratch(seqs, max_q_len, table_width, num_heads, num_kv_heads, block_size, window)
+                             for seqs in (at_once, n_seqs % KV4_SEQS))
         return width, wanted, window, at_once
 
     def attention_kv4_scratch(self, n_seqs: int, n_tokens: int, max_q_len: int, table_width: int, num_heads: int, num_kv_heads: int,

@@ -463,6 +463,24 @@ def test_more_sequences_than_a_launch_takes(n_seqs, most):
         assert bool(((got[mine].double().view(most, 2, 64) - ref).abs() <= HALF_STEP * ref.abs() + 2.0 ** -10 * sums).all())
 
 
+def test_the_last_launch_may_be_cut_in_another_way():
+    """1,024 sequences that need no scratch, and 19 that do."""
+    k = lib(64)
+    n_seqs, heads, kv, most = 1043, 64, 8, 2
+    sizes = (most, 64, heads, kv, 16, 0)
+    assert k.lib.skv_attention_kv4_scratch(1024, *sizes) == 0 and k.lib.skv_attention_kv4_scratch(19, *sizes) > 0
+    cache, table = make_cache(kv, 64, 16, [1024, 1024])
+    table = table[torch.arange(n_seqs, device="cuda") % 2].contiguous()
+    lengths = [1024 - (13 * i) % 700 for i in range(n_seqs)]
+    q = torch.randn(n_seqs * most, heads * 64, device="cuda").bfloat16()
+    got = run_step(k, q, cache, table, [most * i for i in range(n_seqs + 1)], lengths, heads, kv, 64, 16, most)
+    for s in (0, 1023, 1024, n_seqs - 1):
+        mine = slice(most * s, most * (s + 1))
+        ref, sums, _ = plain_kv4.attention(q[mine].double().view(most, heads, 64), cached(cache, table, s, lengths[s], 16, 0),
+                                           cached(cache, table, s, lengths[s], 16, 1), lengths[s] - most, 0.125)
+        assert bool(((got[mine].double().view(most, heads, 64) - ref).abs() <= HALF_STEP * ref.abs() + 2.0 ** -10 * sums).all())
+
+
 def test_a_captured_step_follows_its_inputs():
     """A replayed graph reads lengths, tables and rows as they are then; two graphs with a scratch each, on another stream than the capture's."""
     k = lib(128)
