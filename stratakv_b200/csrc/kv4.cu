@@ -124,27 +124,39 @@ kv4_append_odd_kernel(const float* __restrict__ qkv, const float* __restrict__ c
 
 // Blocks of the cache as the bfloat16 numbers they stand for.  Block i of sequence s is its logical block first + i, where `first` holds
 // the oldest of the last `keep` positions (0: all of them); rows behind the sequence's end are zero.  out_table[s][b] is where logical
-// block b went (0 for those before the first, which nobody may read).
+// block b went (0 for one that went nowhere: that is the first sequence's).
+// With cu_q, what a sequence's own new tokens see through a window, for a kernel that reads whole tiles of `tile` positions: `first` is the block where the
+// tile of the oldest such position begins, and rows ahead of that position are zero as those behind the end are.  What left the window may have been given
+// back and be another sequence's by now, and a tile multiplies its values with probabilities of zero, which make a NaN of a NaN; for the same reason an entry that went nowhere
+// names the first of its own sequence.
 constexpr int UNPACK_THREADS = 256, UNPACK_ITEMS = 4;          // words of eight codes that a thread has on their way at once
 
 __global__ void __launch_bounds__(UNPACK_THREADS)
 kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ k_scale,
                   const uint8_t* __restrict__ v_scale, const int* __restrict__ block_table, int table_width,
                   const int* __restrict__ ctx_after, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
-                  int* __restrict__ out_table, int out_width, int num_kv_heads, int head_dim, int block_size, int keep) {
+                  int* __restrict__ out_table, int out_width, int num_kv_heads, int head_dim, int block_size, int keep, const int* __restrict__ cu_q,
+                  int most_new, int window, int tile) {
     pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.x / out_width, i = blockIdx.x - seq * out_width, kv_head = blockIdx.y;
     const int ctx = ctx_after[seq];
-    const int first = keep > 0 ? max(0, ctx - keep) / block_size : 0, logical = first + i;
+    int first = keep > 0 ? max(0, ctx - keep) / block_size : 0, oldest = 0, nowhere = 0;
+    if (cu_q) {
+        const int q_len = max(0, min(cu_q[seq + 1] - cu_q[seq], most_new));
+        oldest = window > 0 ? (int)max(0ll, (long long)ctx - q_len - window + 1) : 0;
+        first = oldest / tile * tile / block_size;
+        nowhere = seq * out_width;
+    }
+    const int logical = first + i;
     if (kv_head == 0 && blockIdx.z == 0) {
         if (threadIdx.x == 0 && logical < table_width) out_table[(size_t)seq * table_width + logical] = blockIdx.x;
         if (i == 0)
             for (int b = threadIdx.x; b < table_width; b += UNPACK_THREADS)
-                if (b < first || b >= first + out_width) out_table[(size_t)seq * table_width + b] = 0;
+                if (b < first || b >= first + out_width) out_table[(size_t)seq * table_width + b] = nowhere;
     }
-    const int rows = min(block_size, ctx - logical * block_size);          // live rows of this block (none: not positive)
-    const int block = logical < table_width && rows > 0 ? block_table[(size_t)seq * table_width + logical] : 0;
+    const int begin = max(0, oldest - logical * block_size), rows = min(block_size, ctx - logical * block_size);      // live rows of this block
+    const int block = logical < table_width && rows > begin ? block_table[(size_t)seq * table_width + logical] : 0;
     const size_t from = ((size_t)block * num_kv_heads + kv_head) * block_size;
     const size_t to = ((size_t)blockIdx.x * num_kv_heads + kv_head) * block_size;
     const int words = head_dim >> 3, of_one = block_size * words;          // words of eight numbers
@@ -158,7 +170,7 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
             const int idx = first_item + u * UNPACK_THREADS;
             const bool value = idx >= of_one;
             const int at = idx - (value ? of_one : 0), row = at / words, w = at - row * words;
-            const bool live = idx < 2 * of_one && row < rows;
+            const bool live = idx < 2 * of_one && row >= begin && row < rows;
             word[u] = live ? *(const uint32_t*)((value ? v_codes : k_codes) + (from + row) * (head_dim >> 1) + 4 * w) : 0u;
             byte[u] = live ? (value ? v_scale : k_scale)[(from + row) * (head_dim >> 4) + (w >> 1)] : 0u;
             target[u] = (to + row) * head_dim + 8 * w;
@@ -167,7 +179,7 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
         for (int u = 0; u < ITEMS; ++u) {
             const int idx = first_item + u * UNPACK_THREADS;
             if (idx >= 2 * of_one) break;
-            const float s = kv4_scale(byte[u]);                            // (0 behind the sequence's end, and so is all that it scales)
+            const float s = kv4_scale(byte[u]);                            // (0 where no row is live, and so is all that it scales)
             uint32_t packed[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -210,24 +222,42 @@ SKV_EXPORT int skv_append_kv4(const float* qkv, const float* cos_sin, const int*
                       num_heads, num_kv_heads, head_dim, block_size, write_kv, quads_magic);
 }
 
+static int unpack_kv4(const char* name, const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int* block_table,
+                      int table_width, const int* ctx_after, void* k_out, void* v_out, int* out_table, int n_seqs, int out_width, int num_kv_heads,
+                      int head_dim, int block_size, int keep, const int* cu_q, int most_new, int window, int tile, cudaStream_t stream) {
+    if (n_seqs <= 0 || out_width <= 0) return 0;
+    if (head_dim <= 0 || head_dim % KV4_GROUP != 0) return fail(name, "the head size must be a positive multiple of 16");
+    if (block_size <= 0 || block_size % 16 != 0) return fail(name, "block_size must be a positive multiple of 16");
+    if (num_kv_heads <= 0 || num_kv_heads > 65535) return fail(name, "between 1 and 65,535 kv heads are needed");
+    if (keep < 0) return fail(name, "the positions to keep must not be negative");
+    if ((long long)n_seqs * out_width > 0x7fffffffLL) return fail(name, "too many blocks");
+    if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
+        return fail(name, "operands must be 16-byte aligned");
+    const long long items = 2ll * block_size * (head_dim / 8);
+    if (items > 0x40000000ll) return fail(name, "a cache block is too large");
+    const long long wanted = (items + UNPACK_ITEMS * UNPACK_THREADS - 1) / (UNPACK_ITEMS * UNPACK_THREADS), parts = wanted < 64 ? wanted : 64;
+    return launch_pdl(name, kv4_unpack_kernel, dim3((unsigned)(n_seqs * out_width), (unsigned)num_kv_heads, (unsigned)parts), dim3(UNPACK_THREADS), 0,
+                      stream, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table,
+                      table_width, ctx_after, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_table, out_width, num_kv_heads, head_dim,
+                      block_size, keep, cu_q, most_new, window, tile);
+}
+
 SKV_EXPORT int skv_unpack_kv4(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int* block_table,
                               int table_width, const int* ctx_after, void* k_out, void* v_out, int* out_table, int n_seqs, int out_width,
                               int num_kv_heads, int head_dim, int block_size, int keep, cudaStream_t stream) {
-    if (n_seqs <= 0 || out_width <= 0) return 0;
-    if (head_dim <= 0 || head_dim % KV4_GROUP != 0) return fail("skv_unpack_kv4", "the head size must be a positive multiple of 16");
-    if (block_size <= 0 || block_size % 16 != 0) return fail("skv_unpack_kv4", "block_size must be a positive multiple of 16");
-    if (num_kv_heads <= 0 || num_kv_heads > 65535) return fail("skv_unpack_kv4", "between 1 and 65,535 kv heads are needed");
-    if (keep < 0) return fail("skv_unpack_kv4", "the positions to keep must not be negative");
-    if ((long long)n_seqs * out_width > 0x7fffffffLL) return fail("skv_unpack_kv4", "too many blocks");
-    if (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
-        return fail("skv_unpack_kv4", "operands must be 16-byte aligned");
-    const long long items = 2ll * block_size * (head_dim / 8);
-    if (items > 0x40000000ll) return fail("skv_unpack_kv4", "a cache block is too large");
-    const long long wanted = (items + UNPACK_ITEMS * UNPACK_THREADS - 1) / (UNPACK_ITEMS * UNPACK_THREADS), parts = wanted < 64 ? wanted : 64;
-    return launch_pdl("skv_unpack_kv4", kv4_unpack_kernel, dim3((unsigned)(n_seqs * out_width), (unsigned)num_kv_heads, (unsigned)parts), dim3(UNPACK_THREADS), 0,
-                      stream, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table,
-                      table_width, ctx_after, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_table, out_width, num_kv_heads, head_dim,
-                      block_size, keep);
+    return unpack_kv4("skv_unpack_kv4", k_codes, v_codes, k_scale, v_scale, block_table, table_width, ctx_after, k_out, v_out, out_table, n_seqs, out_width,
+                      num_kv_heads, head_dim, block_size, keep, nullptr, 0, 0, 1, stream);
+}
+
+// What the new tokens cu_q[s] .. cu_q[s + 1] - 1 of a sequence (at most most_new of them) see through a window (0: none), for a reader of tiles of `tile` positions.
+SKV_EXPORT int skv_unpack_kv4_seen(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const int* block_table,
+                                   int table_width, const int* ctx_after, void* k_out, void* v_out, int* out_table, int n_seqs, int out_width,
+                                   int num_kv_heads, int head_dim, int block_size, const int* cu_q, int most_new, int window, int tile,
+                                   cudaStream_t stream) {
+    if (n_seqs > 0 && out_width > 0 && (!cu_q || most_new < 0 || window < 0 || tile <= 0))
+        return fail("skv_unpack_kv4_seen", "the tokens' offsets and a positive tile are needed, most_new and window must not be negative");
+    return unpack_kv4("skv_unpack_kv4_seen", k_codes, v_codes, k_scale, v_scale, block_table, table_width, ctx_after, k_out, v_out, out_table, n_seqs,
+                      out_width, num_kv_heads, head_dim, block_size, 0, cu_q, most_new, window, tile, stream);
 }
 
 SKV_EXPORT int skv_has_kv4() { return 1; }
@@ -242,6 +272,11 @@ SKV_EXPORT int skv_append_kv4(const float*, const float*, const int*, const int*
 SKV_EXPORT int skv_unpack_kv4(const void*, const void*, const void*, const void*, const int*, int, const int*, void*, void*, int*, int, int,
                               int, int, int, int, cudaStream_t) {
     return skv::fail("skv_unpack_kv4", "a 4-bit cache is built for bfloat16");
+}
+
+SKV_EXPORT int skv_unpack_kv4_seen(const void*, const void*, const void*, const void*, const int*, int, const int*, void*, void*, int*, int, int, int,
+                                   int, int, const int*, int, int, int, cudaStream_t) {
+    return skv::fail("skv_unpack_kv4_seen", "a 4-bit cache is built for bfloat16");
 }
 
 SKV_EXPORT int skv_has_kv4() { return 0; }

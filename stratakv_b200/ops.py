@@ -33,6 +33,7 @@ LOW_RANK_PLAIN, LOW_RANK_LOG_SIGMOID, LOW_RANK_SOFTPLUS = 0, 1, 2
 # the memories of ``matrix_step`` (csrc/channel_state.cu)
 STEP_CHANNEL, STEP_DELTA, STEP_EXP = 0, 1, 2
 KV4_SEQS = 1024            # sequences that one launch of it takes (csrc/attention_kv4.cu)
+PREFILL_TILE = 64          # positions of a tile of keys (csrc/attention_prefill_tc.cu)
 KV4_UNPACKED = 1 << 30     # bytes of a 4-bit cache's sequences that are read back at once (or one sequence's, if those are more)
 MAX_STREAMS = 8            # copies of the residual stream that ``stream_mix`` takes (csrc/stream_mix.cu)
 
@@ -1462,6 +1463,7 @@ class Kernels:
         p, i = ctypes.c_void_p, ctypes.c_int
         self.lib.skv_append_kv4.argtypes = [p] * 5 + [i] + [p] * 5 + [i] * 6 + [p]
         self.lib.skv_unpack_kv4.argtypes = [p] * 5 + [i] + [p] * 4 + [i] * 6 + [p]
+        self.lib.skv_unpack_kv4_seen.argtypes = [p] * 5 + [i] + [p] * 4 + [i] * 5 + [p] + [i] * 3 + [p]
         self.lib.skv_attention_kv4.argtypes = [p] * 6 + [i] + [p] * 4 + [ctypes.c_longlong] + [i] * 6 + [ctypes.c_float, i, p]
         self.lib.skv_attention_kv4_scratch.argtypes = [i] * 7
         self.lib.skv_attention_kv4_scratch.restype = ctypes.c_longlong
@@ -1515,7 +1517,9 @@ class Kernels:
         """The blocks of each sequence as the bfloat16 numbers they stand for (exactly): ``k_out`` and ``v_out``
         ``[sequences * width, kv_heads, block_size, head_dim]`` get ``width`` blocks of each, from the one that holds the oldest of its last
         ``keep`` positions on (0: from its first block on); rows behind a sequence's end become zero.  ``out_table`` (int32, as
-        ``block_table``) says where each logical block went, for attention over ``k_out`` and ``v_out``."""
+        ``block_table``) says where each logical block went, for attention over ``k_out`` and ``v_out``; blocks that were not read back have 0, which
+        is the first sequence's.  (``attention_prefill_tc`` reads whole tiles of 64 positions and multiplies what is masked in them by zero, so that a NaN
+        there counts: with smaller blocks, ``keep`` has to reach back to a multiple of 64.)"""
         u8, i32 = torch.uint8, torch.int32
         self._want_all("unpack_kv4", (k_codes, u8, "k_codes"), (v_codes, u8, "v_codes"), (k_scale, u8, "k_scale"), (v_scale, u8, "v_scale"),
                        (block_table, i32, "block_table"), (ctx_after, i32, "ctx_after"), (k_out, self.dtype, "k_out"),
@@ -1569,7 +1573,9 @@ class Kernels:
         width, at_once, tiles = 0, min(n_seqs, KV4_SEQS), -(-max_q_len // 128)
         if (not self._kv4_few(n_seqs, max_q_len, num_heads // max(1, num_kv_heads), num_kv_heads, table_width * block_size, self._kv4_sms)
                 and block_size & (block_size - 1) == 0 and block_size >= 16 and self.has_attention_prefill_tc() and head_dim == self.head_dim and tiles <= 65535):
-            width = table_width if window == 0 else min(table_width, (window + max_q_len - 1 + block_size - 2) // block_size + 1)
+            # (whole tiles: a sequence's last window + max_q_len - 1 positions may begin and end anywhere in one)
+            whole = max(block_size, PREFILL_TILE)
+            width = table_width if window == 0 else min(table_width, ((window + max_q_len - 1 + whole - 2) // whole + 1) * (whole // block_size))
         if width:
             # every sequence has room for the longest: a long one among many short ones must not ask for many times the cache
             each = 4 * width * num_kv_heads * block_size * head_dim + 4 * table_width
@@ -1616,10 +1622,10 @@ class Kernels:
                 values = keys + 2 * seqs * width * num_kv_heads * block_size * head_dim
                 table = values + 2 * seqs * width * num_kv_heads * block_size * head_dim
                 lengths = ctx_after.data_ptr() + 4 * at
-                self._check(self.lib.skv_unpack_kv4(
+                self._check(self.lib.skv_unpack_kv4_seen(
                     k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr() + 4 * at * table_width,
                     table_width, lengths, keys, values, table, seqs, width, num_kv_heads, head_dim, block_size,
-                    window + max_q_len - 1 if window > 0 else 0, _stream()), "unpack_kv4")
+                    cu_q.data_ptr() + 4 * at, max_q_len, window, PREFILL_TILE, _stream()), "unpack_kv4")
                 self._check(self.lib.skv_attention_prefill_tc_extras(
                     _ptr(q), pointer(keys), pointer(values), seqs * width, pointer(table), table_width, pointer(cu_q.data_ptr() + 4 * at),
                     pointer(lengths), _ptr(out), seqs, n, max_q_len, num_heads, num_kv_heads, head_dim, block_size, ctypes.c_float(scale), window,

@@ -569,3 +569,59 @@ def test_refusals():
         k.unpack_kv4(*cache, table, ints([40]), blocks, blocks.clone(), torch.empty_like(table), 2, 64, 16, -1)
     with pytest.raises(KernelError, match="results must be"):
         k.unpack_kv4(*cache, table, ints([40]), blocks, blocks[:2].contiguous(), torch.empty_like(table), 2, 64, 16)
+
+
+# ---- sequences of one call ----------------------------------------------------------------------------------------------
+
+def windowed_prompts(dim, block, before, new, window, heads=4, kv=2):
+    """Prompts of unequal length and what run_step wants of them; ``oldest``: the first position that each sequence's queries see."""
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, dim, block, lengths)
+    cu = [0]
+    for c in new:
+        cu.append(cu[-1] + c)
+    q = torch.randn(cu[-1], heads * dim, device="cuda").bfloat16()
+    return cache, table, cu, lengths, [max(0, b - window + 1) for b in before], q
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("block", [16, 32, 64])
+def test_what_is_not_finite_stays_in_its_sequence(monkeypatch, dim, block):
+    """Prompts with a window: the prompt kernel's tiles of 64 keys begin and end outside of the blocks that a sequence's queries see.  A first sequence
+    of nothing but NaN, blocks behind a window that others have taken since, and positions that have left it: none reaches another result."""
+    take(monkeypatch, False)
+    heads, kv, window, before, new = 4, 2, 100, [500, 530, 37, 300], [200, 130, 200, 1]
+    cache, table, cu, lengths, oldest, q = windowed_prompts(dim, block, before, new, window)
+    clean = run_step(lib(dim), q, cache, table, cu, lengths, heads, kv, dim, block, max(new), window)
+    for s in range(4):
+        mine = slice(cu[s], cu[s + 1])
+        ref, sums, whole = plain_kv4.attention(q[mine].double().view(new[s], heads, dim), cached(cache, table, s, lengths[s], block, 0),
+                                               cached(cache, table, s, lengths[s], block, 1), before[s], 1.0 / math.sqrt(dim), window)
+        allowed = HALF_STEP * ref.abs() + (2.0 ** -8 + 2.0 ** -11) * sums + 2.0 ** -32 * whole
+        assert bool(((clean[mine].double().view(new[s], heads, dim) - ref).abs() <= allowed).all()), s
+    spoiled = [c.clone() for c in cache]
+    for of in (2, 3):
+        spoiled[of][table[0, :-(-lengths[0] // block)].long()] = plain_kv4.NOT_FINITE
+        for s in (1, 2, 3):
+            kept, inside = oldest[s] // block, oldest[s] % block
+            spoiled[of][table[s, kept].long(), :, :inside] = plain_kv4.NOT_FINITE
+    moved = table.clone()
+    for s in (1, 2, 3):
+        moved[s, :oldest[s] // block] = table[0, 0]
+    got = run_step(lib(dim), q, spoiled, moved, cu, lengths, heads, kv, dim, block, max(new), window)
+    assert bool(torch.isnan(got[:cu[1]]).all())
+    assert torch.equal(got[cu[1]:], clean[cu[1]:])
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("few", [False, True])
+def test_entries_of_blocks_that_nobody_sees_are_not_read(monkeypatch, block, few):
+    """Behind a window and behind a sequence's end a table may hold anything."""
+    take(monkeypatch, few)
+    heads, kv, dim, window, before, new = 4, 2, 64, 100, [500, 530, 37, 300], [200, 130, 200, 1]
+    cache, table, cu, lengths, oldest, q = windowed_prompts(dim, block, before, new, window)
+    clean = run_step(lib(dim), q, cache, table, cu, lengths, heads, kv, dim, block, max(new), window)
+    for s in range(4):
+        table[s, :oldest[s] // block] = -2 ** 31
+        table[s, -(-lengths[s] // block):] = 2 ** 31 - 1
+    assert torch.equal(run_step(lib(dim), q, cache, table, cu, lengths, heads, kv, dim, block, max(new), window), clean)
