@@ -224,12 +224,18 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const int head = blockIdx.x;
     const int kv_head = head / (num_heads / num_kv_heads);
     pdl_launch_dependents();
+    // (A block that has nothing to do waits all the same: a grid of such blocks alone would be complete ahead of the kernel in front of it, and the
+    // kernel behind, which waits for this one only, would run beside that.)
     if (a_smem(a_raw) & 1023) {
         if (threadIdx.x == 0 && flag) atomicOr(flag, 4);
+        pdl_wait();
         return;
     }
     const int q_begin = cu_q[seq], q_len = cu_q[seq + 1] - q_begin;
-    if (tile * ABM >= q_len) return;                               // the whole block leaves together
+    if (tile * ABM >= q_len) {                                     // the whole block leaves together
+        pdl_wait();
+        return;
+    }
     const int ctx = ctx_after[seq], ctx_before = ctx - q_len;
     const int last_query = min(q_len, tile * ABM + ABM) - 1;
     const int kv_end = ctx_before + last_query + 1;

@@ -2,6 +2,7 @@
 import ctypes
 import dataclasses
 import math
+import re
 
 import pytest
 import torch
@@ -186,3 +187,31 @@ def test_float32_libraries_have_none():
     assert lib.skv_attention_kv4(null, null, null, null, null, null, i(1), null, null, null, null, ctypes.c_longlong(0), i(1), i(1), i(1), i(1), i(64),
                                  i(16), ctypes.c_float(1.0), i(0), null) != 0
     assert b"bfloat16" in lib.skv_last_error()
+
+
+def without_lambdas(text):
+    while (at := text.find("[&]")) >= 0:
+        end = start = text.index("{", at)
+        depth = 0
+        while True:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+            if depth == 0:
+                break
+        text = text[:at] + text[end:]
+    return text
+
+
+def test_no_kernel_leaves_ahead_of_its_wait():
+    """A grid whose blocks all return before they wait for the grid in front of them is complete before that one, and whoever waits for it alone runs
+    beside the other: attention over the next piece of a scratch, while the piece before is still written."""
+    seen = 0
+    for path in sorted(build.CSRC.glob("*.cu")):
+        for piece in path.read_text().split("pdl_launch_dependents();")[1:]:
+            body = without_lambdas(piece.split("\n}\n")[0])
+            seen += 1
+            assert "pdl_wait();" in body, path.name
+            for leaving in re.finditer(r"\breturn;", body[:max(0, body.rfind("pdl_wait();"))]):
+                before = body[:leaving.start()].rstrip()
+                assert before.endswith("pdl_wait();") or before.count("pdl_wait();") > before.count("return;"), path.name
+    assert seen > 50

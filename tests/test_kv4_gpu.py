@@ -625,3 +625,28 @@ def test_entries_of_blocks_that_nobody_sees_are_not_read(monkeypatch, block, few
         table[s, :oldest[s] // block] = -2 ** 31
         table[s, -(-lengths[s] // block):] = 2 ** 31 - 1
     assert torch.equal(run_step(lib(dim), q, cache, table, cu, lengths, heads, kv, dim, block, max(new), window), clean)
+
+
+@pytest.mark.parametrize("window", [0, 150])
+def test_prompts_read_back_in_pieces_without_new_tokens(monkeypatch, window):
+    """Pieces all of whose sequences bring no token between pieces that bring some, one sequence at a time through one scratch: nobody's keys are
+    written over while they are read."""
+    from stratakv_b200 import ops
+    k = lib(64)
+    heads, kv, block, before, new = 8, 2, 64, [900, 2000, 2000, 40, 700, 2000, 300], [200, 0, 0, 200, 130, 0, 170]
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, 64, block, lengths)
+    cu = [0]
+    for c in new:
+        cu.append(cu[-1] + c)
+    q = torch.randn(cu[-1], heads * 64, device="cuda").bfloat16()
+    take(monkeypatch, False)
+    whole = k.attention_kv4_scratch(7, cu[-1], 200, table.shape[1], heads, kv, 64, block, window)
+    monkeypatch.setattr(ops, "KV4_UNPACKED", whole // 7)
+    assert k.attention_kv4_scratch(7, cu[-1], 200, table.shape[1], heads, kv, 64, block, window) == whole // 7
+    alone = {s: run_step(k, q[cu[s]:cu[s + 1]].contiguous(), cache, table[s:s + 1].contiguous(), [0, new[s]], [lengths[s]], heads, kv, 64, block, 200, window)
+             for s in range(7) if new[s]}
+    for _ in range(20):
+        got = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
+        for s, result in alone.items():
+            assert torch.equal(got[cu[s]:cu[s + 1]], result), s
