@@ -41,7 +41,9 @@ class EngineConfig:
     capacity (``src/generation/generator.cpp:628-632``).  ``cache_dtype``: what keys
     and values are kept in, the compute dtype ("" or its name) or "int4": 4 bits and
     a scale byte for each 16 numbers, 0.28 of bfloat16's bytes (bfloat16 models all
-    of whose cached layers are plain attention)."""
+    of whose cached layers are plain attention).  Prompts read such a cache back into
+    workspace beside it: up to 1 GB, or one sequence's keys and values of one layer in
+    bfloat16 where those are more."""
     max_tokens: int
     dtype: torch.dtype = torch.bfloat16
     block_size: int = 64

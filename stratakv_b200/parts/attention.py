@@ -396,7 +396,7 @@ class PagedAttention(Mixer):
                        s.num_kv_heads, s.head_dim, block_size, writes_cache)
         wanted = ops.attention_kv4_scratch(step.n_seqs, n, step.max_q_len, table.shape[1], s.num_heads, s.num_kv_heads, s.head_dim,
                                            block_size, s.window)
-        scratch = rt.workspace.get("kv4_scratch", (wanted,), torch.uint8) if wanted else None
+        scratch = rt.workspace.get("kv4_scratch", (wanted,), torch.uint8, most=_ops.KV4_UNPACKED) if wanted else None
         ops.attention_kv4(q, *cache, table, step.cu_q, step.ctx_after, ctx, step.max_q_len, s.num_heads, s.num_kv_heads, s.head_dim,
                           block_size, s.scale, s.window, scratch)
 

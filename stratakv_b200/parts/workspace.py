@@ -17,8 +17,9 @@ class Workspace:
         self._views: Dict[Tuple[str, torch.dtype], Tuple[tuple, torch.Tensor]] = {}
         self.generation = 0          # bumped whenever a buffer is reallocated
 
-    def get(self, name: str, shape, dtype: torch.dtype, zero: bool = False) -> torch.Tensor:
-        """``zero``: the buffer is zero when it is first handed out (and after it had to grow)."""
+    def get(self, name: str, shape, dtype: torch.dtype, zero: bool = False, most: int = 0) -> torch.Tensor:
+        """``zero``: the buffer is zero when it is first handed out (and after it had to grow).  A buffer that has to grow
+        doubles, with ``most`` > 0 up to so many elements (or what is asked for); the old one is gone before the new one is made."""
         key = (name, dtype)
         last = self._views.get(key)
         if last is not None and last[0] == shape:
@@ -30,7 +31,11 @@ class Workspace:
         if buffer is None or buffer.numel() < count:
             capacity = max(count, 1)
             if buffer is not None:
-                capacity = max(capacity, 2 * buffer.numel())
+                doubled = 2 * buffer.numel()
+                capacity = max(capacity, min(doubled, most) if most > 0 else doubled)
+                del self._buffers[key]
+                self._views.pop(key, None)
+                buffer = last = None
             buffer = (torch.zeros if zero else torch.empty)(capacity, dtype=dtype, device=self.device)
             self._buffers[key] = buffer
             self.generation += 1

@@ -215,3 +215,49 @@ def test_no_kernel_leaves_ahead_of_its_wait():
                 before = body[:leaving.start()].rstrip()
                 assert before.endswith("pdl_wait();") or before.count("pdl_wait();") > before.count("return;"), path.name
     assert seen > 50
+
+
+def test_scratch_grows_within_its_bound(monkeypatch):
+    """A buffer with a bound doubles up to it, takes what is asked for beyond, and is gone before the larger one is made."""
+    import weakref
+    from stratakv_b200.parts.workspace import Workspace
+    made, real = [], torch.empty
+
+    def empty(count, **options):
+        assert all(old() is None for _, old in made)
+        tensor = real(count, **options)
+        made.append((count, weakref.ref(tensor)))
+        return tensor
+
+    workspace = Workspace("cpu")
+    monkeypatch.setattr(torch, "empty", empty)
+    for count in (100, 90, 150, 700, 1400, 1500, 1600, 1550, 3000, 20):
+        assert workspace.get("scratch", (count,), torch.uint8, most=1600).numel() == count
+    assert [count for count, _ in made] == [100, 200, 700, 1400, 1600, 3000] and workspace.generation == 6
+    made.clear()
+    for count in (100, 150, 250):                          # (without a bound: twice as much)
+        workspace.get("rows", (count,), torch.float32)
+    assert [count for count, _ in made] == [100, 200, 400]
+
+
+def test_prompts_ask_for_scratch_within_its_bound():
+    """What the mixer asks its workspace for: a bound of 1 GB beside the bytes of the step."""
+    from types import SimpleNamespace
+    from stratakv_b200 import ops
+    from stratakv_b200.parts.attention import PagedAttention
+    asked = {}
+
+    def get(name, shape, dtype, zero=False, most=0):
+        asked[name] = (shape, most)
+        return torch.empty(shape, dtype=dtype)
+
+    wanted = [3000]
+    kernels = SimpleNamespace(append_kv4=lambda *a: None, attention_kv4=lambda *a: None, attention_kv4_scratch=lambda *a: wanted[0])
+    cache = SimpleNamespace(block_size=64, entry_storage=lambda e: {"k": 0, "v": 0, "k_scale": 0, "v_scale": 0}, entry_group_index=lambda e: 0)
+    step = SimpleNamespace(cache=cache, block_tables={0: torch.zeros(1, 5)}, max_ctx=300, positions=None, token_seq=None, n_seqs=1, max_q_len=300, cu_q=None,
+                           ctx_after=None)
+    mixer = SimpleNamespace(spec=SimpleNamespace(num_heads=4, num_kv_heads=2, head_dim=64, window=0, scale=0.125), q_dim=256,
+                            rt=SimpleNamespace(kernels=lambda dim: kernels, dtype=torch.bfloat16, workspace=SimpleNamespace(get=get)),
+                            position=SimpleNamespace(fusion_table=lambda n: None))
+    PagedAttention._attend_in_4_bits(mixer, step, torch.zeros(300, 512), None, 0, True)
+    assert asked["kv4_scratch"] == ((3000,), ops.KV4_UNPACKED)
