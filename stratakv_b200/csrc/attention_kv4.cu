@@ -2,8 +2,9 @@
 //
 // The mathematics is that of attention_decode.cu: scores (q.k) * scale over the sequence's visible positions, a softmax whose maximum
 // and sum run along with one pass over the keys, and the weighted sum of values, in float.  The products take half precision,
-// in which what the cache holds is exact: a query is brought to a largest magnitude between 1 and 2 by a power of two (its 8
-// bits fit a half's 11), and the probabilities keep 11 bits.
+// in which what the cache holds is exact: a query head is brought to a largest magnitude between 2^15 and 2^16 by a power of two (a half
+// ends at 65,504, a bfloat16 below 2^16 at 65,280), so that its numbers down to 2^-32 of the largest keep their 8 bits and smaller ones are
+// off by 2^-40 of it at most; and the probabilities keep 11 bits.
 //
 // An item is a key head of a sequence and up to 8 NT rows (a row: a query head of one new token; the heads that share a key head lie side by side); a warp
 // takes 32 keys of it at a time (16 where a cache block is no multiple of 32), which asynchronous copies have brought to its own part of shared memory.
@@ -331,8 +332,8 @@ kv4_attention_kernel(const __nv_bfloat16* __restrict__ q, const uint8_t* __restr
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         finite = (__ballot_sync(0xffffffffu, finite) >> (lane & 28) & 15u) == 15u;
-        // most = 2^power (1 + ...); what is not finite stays so in a half
-        const int power = most > 0.0f && finite ? min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 126) : 0;
+        // most = 2^(power + 15) (1 + ...); what is not finite stays so in a half
+        const int power = most > 0.0f && finite ? max((int)(__float_as_uint(most) >> 23) - 127 - 15, -115) : 0;          // (at most 112)
         const float down = __uint_as_float((uint32_t)(127 - power) << 23);
 #pragma unroll
         for (int j = 0; j < KWORDS; ++j) {

@@ -650,3 +650,31 @@ def test_prompts_read_back_in_pieces_without_new_tokens(monkeypatch, window):
         got = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
         for s, result in alone.items():
             assert torch.equal(got[cu[s]:cu[s + 1]], result), s
+
+
+@pytest.mark.parametrize("power", [10, 17, 24, 30, 120])
+@pytest.mark.parametrize("dim,few", [(64, True), (128, True), (80, True), (64, False), (128, False)])
+def test_queries_of_a_wide_range(monkeypatch, dim, few, power):
+    """A number of a query head that is many times the others and meets zeros: what the others say decides.  A number of the head is off by at most
+    2^-40 of the power of two below the largest, as a half's last place is 2^-24 and the largest is brought to 2^15."""
+    take(monkeypatch, few)
+    k = lib(dim)
+    heads, kv, block, before, new = 4, 2, 16, [400, 90], [3, 2]
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, dim, block, lengths, spread=3.0)
+    cache[0][..., 0] = cache[0][..., 0] & 0xF0 | 8                # (number 0 of every key: 0)
+    cu = [0, new[0], sum(new)]
+    q = torch.randn(cu[-1], heads * dim, device="cuda").bfloat16()
+    q[:, 0::dim] = 2.0 ** power * 1.9921875
+    got = run_step(k, q, cache, table, cu, lengths, heads, kv, dim, block, max(new))
+    for s in range(2):
+        mine = slice(cu[s], cu[s + 1])
+        keys = cached(cache, table, s, lengths[s], block, 0)
+        rows = q[mine].double().view(new[s], heads, dim)
+        if power > 50:                                            # (the others are below a half's last place)
+            rows = torch.zeros_like(rows) if few else rows
+        ref, sums, whole = plain_kv4.attention(rows, keys, cached(cache, table, s, lengths[s], block, 1), before[s], 1.0 / math.sqrt(dim))
+        # scores off by d change weights by a factor of e^(2 d) at most
+        off = 2.0 ** (power - 40) * float(keys.abs().sum(-1).max()) / math.sqrt(dim) if few and power < 50 else 0.0
+        allowed = HALF_STEP * ref.abs() + ((2.0 ** -11 if few else 2.0 ** -8) + 2.0 ** -11 + math.expm1(2 * off)) * sums + 2.0 ** -32 * whole
+        assert bool(((got[mine].double().view(new[s], heads, dim) - ref).abs() <= allowed).all()), (s, off)
