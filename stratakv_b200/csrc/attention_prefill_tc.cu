@@ -236,7 +236,7 @@ prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         pdl_wait();
         return;
     }
-    const int ctx = ctx_after[seq], ctx_before = ctx - q_len;
+    const int ctx = (int)min((long long)ctx_after[seq], (long long)table_width * block_size), ctx_before = ctx - q_len;      // (a length beyond the table is cut)
     const int last_query = min(q_len, tile * ABM + ABM) - 1;
     const int kv_end = ctx_before + last_query + 1;
     const int kv_lo = window > 0 ? max(0, ctx_before + tile * ABM - window + 1) : 0;

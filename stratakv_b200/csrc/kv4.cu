@@ -140,7 +140,7 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
     pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.x / out_width, i = blockIdx.x - seq * out_width, kv_head = blockIdx.y;
-    const int ctx = ctx_after[seq];
+    const int ctx = cu_q ? (int)min((long long)ctx_after[seq], (long long)table_width * block_size) : ctx_after[seq];     // (for attention a length beyond the table is cut)
     int first = keep > 0 ? max(0, ctx - keep) / block_size : 0, oldest = 0, nowhere = 0;
     if (cu_q) {
         const int q_len = max(0, min(cu_q[seq + 1] - cu_q[seq], most_new));

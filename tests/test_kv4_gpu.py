@@ -678,3 +678,20 @@ def test_queries_of_a_wide_range(monkeypatch, dim, few, power):
         off = 2.0 ** (power - 40) * float(keys.abs().sum(-1).max()) / math.sqrt(dim) if few and power < 50 else 0.0
         allowed = HALF_STEP * ref.abs() + ((2.0 ** -11 if few else 2.0 ** -8) + 2.0 ** -11 + math.expm1(2 * off)) * sums + 2.0 ** -32 * whole
         assert bool(((got[mine].double().view(new[s], heads, dim) - ref).abs() <= allowed).all()), (s, off)
+
+
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("block", [16, 64])
+def test_a_length_beyond_the_table_is_cut(monkeypatch, block, few, window):
+    """To the positions that the table has, whichever way a step takes."""
+    take(monkeypatch, few)
+    k = lib(64)
+    heads, kv, before, new = 4, 2, [440, 300, 440], [200, 70, 200]      # (640 positions fill the table)
+    lengths = [b + n for b, n in zip(before, new)]
+    cache, table = make_cache(kv, 64, block, lengths)
+    cu = [0, 200, 270, 470]
+    q = torch.randn(470, heads * 64, device="cuda").bfloat16()
+    clean = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
+    assert bool(torch.isfinite(clean).all())
+    assert torch.equal(run_step(k, q, cache, table, cu, [641, 370, 10 ** 5], heads, kv, 64, block, 200, window), clean)
