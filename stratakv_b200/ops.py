@@ -7,6 +7,7 @@ raise; nothing falls back to the CPU or to library model code.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from typing import Dict, Optional, Tuple
 
@@ -1595,7 +1596,7 @@ class Kernels:
     def attention_kv4(self, q, k_codes, v_codes, k_scale, v_scale, block_table, cu_q, ctx_after, out, max_q_len: int, num_heads: int,
                       num_kv_heads: int, head_dim: int, block_size: int, scale: float, window: int = 0, scratch=None, flag=None):
         """Causal attention over a cache held in 4 bits (bfloat16 build): sequence ``s`` owns rows ``cu_q[s]..cu_q[s+1]-1`` of
-        ``q``/``out`` (at most ``max_q_len``), ``ctx_after[s]`` positions are cached, this step's included.  One or a few new tokens a sequence
+        ``q``/``out`` (at most ``max_q_len``), ``ctx_after[s]`` positions are cached, this step's included; ``scale`` is positive.  One or a few new tokens a sequence
         read the cache as it lies; many read the bfloat16 numbers it stands for (``unpack_kv4``, then
         ``attention_prefill_tc``, by which a value's NaN reaches all queries of a tile, as over a 16-bit cache).  ``scratch``: uint8, at least ``attention_kv4_scratch`` bytes; two steps that may run at once need one each.
         A step's sums are cut by all its sequences' lengths, so that a sequence's result may differ in their order between batches."""
@@ -1609,6 +1610,8 @@ class Kernels:
             raise KernelError("attention_kv4: one length, one offset pair and one table row per sequence is needed")
         if q.shape != (n, num_heads * head_dim) or out.shape != q.shape or max_q_len < 1:
             raise KernelError("attention_kv4: q and out must be [tokens, heads * head_dim]")
+        if not 0.0 < scale < math.inf:
+            raise KernelError("attention_kv4: the scale must be positive and finite")
         width, wanted, window, at_once = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
         if wanted:
             if scratch is None or scratch.numel() < wanted:

@@ -695,3 +695,19 @@ def test_a_length_beyond_the_table_is_cut(monkeypatch, block, few, window):
     clean = run_step(k, q, cache, table, cu, lengths, heads, kv, 64, block, 200, window)
     assert bool(torch.isfinite(clean).all())
     assert torch.equal(run_step(k, q, cache, table, cu, [641, 370, 10 ** 5], heads, kv, 64, block, 200, window), clean)
+
+
+@pytest.mark.parametrize("new", [1, 200])
+@pytest.mark.parametrize("scale", [0.0, -0.125, math.nan, math.inf])
+def test_a_scale_that_is_not_positive_is_refused(monkeypatch, new, scale):
+    """Prompts mask a score by minus infinity ahead of the scale."""
+    from stratakv_b200.ops import KernelError
+    take(monkeypatch, new == 1)
+    k = lib(64)
+    cache, table = make_cache(2, 64, 16, [300 + new])
+    q = torch.randn(new, 4 * 64, device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    scratch = torch.empty(k.attention_kv4_scratch(1, new, new, table.shape[1], 4, 2, 64, 16), dtype=torch.uint8, device="cuda")
+    with pytest.raises(KernelError, match="scale must be positive"):
+        k.attention_kv4(q, *cache, table, ints([0, new]), ints([300 + new]), out, new, 4, 2, 64, 16, scale, 0, scratch)
+    assert bool((out == 7.0).all())
