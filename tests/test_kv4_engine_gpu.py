@@ -116,3 +116,98 @@ def test_the_command_line(folders):
     assert len(result.stdout.split()) <= 8 and result.stdout.split()[:3] == ["3", "1", "4"]
     result = subprocess.run(command[:2] + ["--dtype", "float32"] + command[2:], capture_output=True, text=True, timeout=300)
     assert result.returncode == 1 and "bfloat16 kernels alone" in result.stderr
+
+
+def windowed_engine(window, block_size, max_tokens):
+    import dataclasses
+    from stratakv_b200 import Engine, EngineConfig
+    from stratakv_b200.config import LlamaConfig
+    from stratakv_b200.config.registry import resolve_architecture
+    from stratakv_b200.engine.model import expected_tensors
+    from stratakv_b200.weights.random_init import random_tensors
+    config = LlamaConfig.from_dict(TINY["E"])
+    spec = resolve_architecture(config.architecture).build_spec(config)
+    spec = dataclasses.replace(spec, layers=tuple(dataclasses.replace(layer, mixer=dataclasses.replace(layer.mixer, window=window)) for layer in spec.layers))
+    tensors = random_tensors(expected_tensors(spec), 5, dtype=torch.bfloat16)
+    return Engine(spec, tensors, EngineConfig(max_tokens=max_tokens, block_size=block_size, max_context=4096, cache_dtype="int4"), verbose=False)
+
+
+@pytest.mark.parametrize("direct", [True, False])
+@pytest.mark.parametrize("block", [16, 64])
+def test_a_window_whose_blocks_others_take(monkeypatch, block, direct):
+    """Two sequences through a windowed layer whose cache is so small that what the one's window gives back is the other's next: each attends over its
+    own last positions alone.  ``direct``: prompts read the 4-bit cache too."""
+    from stratakv_b200 import StepEntry, ops
+    window = 40
+    engine = windowed_engine(window, block, 224 if block == 16 else 384)
+    monkeypatch.setattr(ops.Kernels, "_kv4_few", staticmethod(lambda n_seqs, max_q_len, *sizes: direct or max_q_len < 8))
+    mixer = engine.model.layers[0].mixer
+    s = mixer.spec
+    assert s.cache_bits == 4 and s.window == window and engine.cache.groups[0].kind.name == "kv4_window"
+    slots = [engine.open_sequence() for _ in range(2)]
+    before, stored, had = [0, 0], [[], []], [set(), set()]
+    for new in ([90, 20], [1, 1], [1, 60], [100, 1], [1, 100], [1, 1], [3, 2], [1, 1]):
+        step, _, _ = engine.prepare([StepEntry(slot, [1] * c, []) for slot, c in zip(slots, new)])
+        for i, slot in enumerate(slots):
+            had[i] |= set(engine.cache.sequences[slot].blocks[0])
+        n = sum(new)
+        h = torch.randn(n, s.hidden_size, device="cuda").bfloat16()
+        qkv = torch.empty(n, mixer.q_dim + 2 * mixer.kv_dim, device="cuda")
+        engine.rt.kernels(s.head_dim).linear(h, mixer.w_qkv, qkv, ops.MODE_STORE_F32)
+        x = torch.zeros(n, s.hidden_size, device="cuda")
+        mixer.forward(step, h, x, 0, True)
+        rows = qkv.view(n, -1, s.head_dim)
+        turned = plain_kv4.rotate(rows[:, :s.num_heads + s.num_kv_heads], mixer.position.fusion_table(step.max_ctx), step.positions)
+        ctx, allowed, at = [], [], 0
+        for i, c in enumerate(new):
+            mine = slice(at, at + c)
+            stored[i].append([plain_kv4.read(*plain_kv4.store(part[mine])) for part in (turned[:, s.num_heads:], rows[:, s.num_heads + s.num_kv_heads:])])
+            keys, values = (torch.cat([piece[j] for piece in stored[i]]).transpose(0, 1) for j in (0, 1))
+            ref, sums, whole = plain_kv4.attention(turned[mine, :s.num_heads].bfloat16().double(), keys, values, before[i], s.scale, window)
+            ctx.append(ref)
+            # (rounded once; probabilities of 8 bits at worst, sums of products and exponentials 2^-11)
+            allowed.append(2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -11) * sums + 2.0 ** -32 * whole)
+            at += c
+            engine.cache.advance(slots[i], before[i] + c)
+            before[i] += c
+        w = mixer.w_o.double()
+        ctx, allowed = (torch.cat(part).flatten(1) for part in (ctx, allowed))
+        # the projection's own sums: at most heads * head_dim roundings of 2^-24, and the tensor core's cut of 2^-23 per product
+        bound = allowed @ w.abs().T + 2.0 ** -22 * ctx.shape[1] ** 0.5 * (ctx.abs() @ w.abs().T) + 1e-30
+        error = (x.double() - ctx @ w.T).abs()
+        assert bool((error <= bound).all()), (new, float((error / bound).max()))
+    assert had[0] & had[1]
+
+
+def test_decode_steps_keep_to_their_own_sequence(folders):
+    """The same tokens given to sequences in a batch and to each alone: their logits differ by what another order of sums does to the stored codes.
+    bfloat16 rows that differ by a rounding (2^-8 of a number) store another code where they straddle a border of codes: a step is a seventh of a
+    group's largest number, so in up to 7 x 2^-8 of the numbers, 3 %, by a step each, 0.17 of a step in the mean square; the rounding to codes itself
+    is 0.29 of a step.  So this is at most 0.6 of what 4 bits do to a logit, 0.35 of the logits' spread: 0.21.  Another sequence's keys move them by more."""
+    from stratakv_b200 import StepEntry
+    engine = engine_for(folders["E"])
+    lengths = (40, 200, 7)
+    prompts = [random_tokens(300, n, seed=n) for n in lengths]
+    forced = [random_tokens(300, 12, seed=100 + n) for n in lengths]
+
+    def logits_of(prompts, forced):
+        slots = [engine.open_sequence() for _ in prompts]
+        engine.step([StepEntry(slot, p, []) for slot, p in zip(slots, prompts)])
+        got = torch.stack([engine.step([StepEntry(slot, [f[i]], [0]) for slot, f in zip(slots, forced)]).clone() for i in range(12)], dim=1).double()
+        for slot in slots:
+            engine.close_sequence(slot)
+        engine.check_flags()
+        return got
+
+    launched = engine.graph_launches
+    together = logits_of(prompts, forced)
+    assert engine.graph_launches > launched
+    for i, n in enumerate(lengths):
+        alone = logits_of([prompts[i]], [forced[i]])[0]
+        other = logits_of([random_tokens(300, n, seed=50 + n)], [forced[i]])[0]
+        spread = float(alone.std())
+        moved, told = float((together[i] - alone).std()) / spread, float((other - alone).std()) / spread
+        print(f"length {n}: together {moved:.4f}, behind another prompt {told:.4f}")
+        assert moved < 0.21
+        assert told > 2 * moved
+    assert engine.cache.all_free()

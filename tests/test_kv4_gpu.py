@@ -711,3 +711,35 @@ def test_a_scale_that_is_not_positive_is_refused(monkeypatch, new, scale):
     with pytest.raises(KernelError, match="scale must be positive"):
         k.attention_kv4(q, *cache, table, ints([0, new]), ints([300 + new]), out, new, 4, 2, 64, 16, scale, 0, scratch)
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,kv,block,before,new,window", [
+    (6, 2, 64, [0], [1], 0), (6, 2, 16, [299, 16, 40], [1, 1, 1], 0), (16, 16, 32, [70, 500], [1, 1], 33), (24, 1, 64, [600], [3], 0), (4, 4, 48, [90, 0], [50, 7], 0),
+    (8, 2, 32, [0, 77], [200, 130], 100), (6, 2, 64, [17000, 511], [1, 1], 0)])
+def test_attention_of_heads_of_96(heads, kv, block, before, new, window):
+    """(A key's 48 bytes of codes are three pieces, which no power of two of lanes shares out.)"""
+    check_attention(heads, kv, 96, block, before, new, window)
+
+
+def test_append_and_read_back_of_heads_of_96():
+    from stratakv_b200.parts.position import rope_table
+    heads, kv, dim, block, new = 5, 1, 96, 16, [33, 1, 20]
+    k = lib(dim)
+    cache, table = make_cache(kv, dim, block, new)
+    n = sum(new)
+    qkv = torch.randn(n, (heads + 2 * kv) * dim, device="cuda")
+    positions = torch.cat([torch.arange(c) for c in new]).int().cuda()
+    seqs = torch.repeat_interleave(torch.arange(3), torch.tensor(new)).int().cuda()
+    cos_sin = torch.from_numpy(rope_table(dim, 10000.0, 40)).cuda()
+    q_out = torch.empty(n, heads * dim, dtype=torch.bfloat16, device="cuda")
+    k.append_kv4(qkv, cos_sin, positions, seqs, table, q_out, *cache, heads, kv, dim, block)
+    rows = qkv.view(n, heads + 2 * kv, dim)
+    turned = plain_kv4.rotate(rows[:, :heads + kv], cos_sin, positions)
+    assert torch.equal(q_out, turned[:, :heads].flatten(1).bfloat16())
+    out = [torch.empty(table.numel(), kv, block, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    k.unpack_kv4(*cache, table, ints(new), *out, torch.empty_like(table), kv, dim, block)
+    for of, x in ((0, turned[:, heads:]), (1, rows[:, heads + kv:])):
+        plain = plain_kv4.read(*plain_kv4.store(x))
+        got = out[of].view(3, table.shape[1], kv, block, dim).transpose(1, 2).flatten(2, 3)
+        for s, c in enumerate(new):
+            assert torch.equal(got[s, :, :c].double(), plain[seqs == s].transpose(0, 1)) and bool((got[s, :, c:] == 0).all())
