@@ -1612,6 +1612,8 @@ class Kernels:
             raise KernelError("attention_kv4: q and out must be [tokens, heads * head_dim]")
         if not 0.0 < scale < math.inf:
             raise KernelError("attention_kv4: the scale must be positive and finite")
+        if n == 0:                                             # (an empty tensor has no address, which the prompt kernel's tensor maps want)
+            return
         width, wanted, window, at_once = self._kv4_plan(n_seqs, max_q_len, table_width, num_heads, num_kv_heads, head_dim, block_size, window)
         if wanted:
             if scratch is None or scratch.numel() < wanted:

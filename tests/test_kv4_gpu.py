@@ -743,3 +743,12 @@ def test_append_and_read_back_of_heads_of_96():
         got = out[of].view(3, table.shape[1], kv, block, dim).transpose(1, 2).flatten(2, 3)
         for s, c in enumerate(new):
             assert torch.equal(got[s, :, :c].double(), plain[seqs == s].transpose(0, 1)) and bool((got[s, :, c:] == 0).all())
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_a_step_without_any_token(monkeypatch, few):
+    """Sequences, but no rows: nothing to do, whichever way the sizes would take."""
+    take(monkeypatch, few)
+    cache, table = make_cache(2, 64, 64, [300, 40])
+    q = torch.empty(0, 4 * 64, device="cuda", dtype=torch.bfloat16)
+    assert run_step(lib(64), q, cache, table, [0, 0, 0], [300, 40], 4, 2, 64, 64, 200).shape == (0, 256)
