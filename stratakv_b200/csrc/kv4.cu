@@ -125,13 +125,14 @@ kv4_append_odd_kernel(const float* __restrict__ qkv, const float* __restrict__ c
 // Blocks of the cache as the bfloat16 numbers they stand for.  Block i of sequence s is its logical block first + i, where `first` holds
 // the oldest of the last `keep` positions (0: all of them); rows behind the sequence's end are zero.  out_table[s][b] is where logical
 // block b went (0 for one that went nowhere: that is the first sequence's).
-// With cu_q, what a sequence's own new tokens see through a window, for a kernel that reads whole tiles of `tile` positions: `first` is the block where the
+// SEEN: what a sequence's own new tokens see through a window, for a kernel that reads whole tiles of `tile` positions: `first` is the block where the
 // tile of the oldest such position begins, and rows ahead of that position are zero as those behind the end are.  What left the window may have been given
 // back and be another sequence's by now, and a tile multiplies its values with probabilities of zero, which make a NaN of a NaN; for the same reason an entry that went nowhere
 // names the first of its own sequence.
 constexpr int UNPACK_THREADS = 256, UNPACK_ITEMS = 4;          // words of eight codes that a thread has on their way at once
 
-__global__ void __launch_bounds__(UNPACK_THREADS)
+template <bool SEEN>
+__global__ void __launch_bounds__(UNPACK_THREADS, SEEN ? 8 : 0)
 kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes, const uint8_t* __restrict__ k_scale,
                   const uint8_t* __restrict__ v_scale, const int* __restrict__ block_table, int table_width,
                   const int* __restrict__ ctx_after, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
@@ -140,23 +141,25 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
     pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.x / out_width, i = blockIdx.x - seq * out_width, kv_head = blockIdx.y;
-    const int ctx = cu_q ? (int)min((long long)ctx_after[seq], (long long)table_width * block_size) : ctx_after[seq];     // (for attention a length beyond the table is cut)
-    int first = keep > 0 ? max(0, ctx - keep) / block_size : 0, oldest = 0, nowhere = 0;
-    if (cu_q) {
+    // (for attention a length beyond the table is cut)
+    const int ctx = SEEN ? (int)min((long long)ctx_after[seq], (long long)table_width * block_size) : ctx_after[seq];
+    int first = 0, oldest = 0;
+    if (!SEEN) {
+        if (keep > 0) first = max(0, ctx - keep) / block_size;
+    } else if (window > 0) {
         const int q_len = max(0, min(cu_q[seq + 1] - cu_q[seq], most_new));
-        oldest = window > 0 ? (int)max(0ll, (long long)ctx - q_len - window + 1) : 0;
+        oldest = (int)max(0ll, (long long)ctx - q_len - window + 1);
         first = oldest / tile * tile / block_size;
-        nowhere = seq * out_width;
     }
     const int logical = first + i;
     if (kv_head == 0 && blockIdx.z == 0) {
         if (threadIdx.x == 0 && logical < table_width) out_table[(size_t)seq * table_width + logical] = blockIdx.x;
         if (i == 0)
             for (int b = threadIdx.x; b < table_width; b += UNPACK_THREADS)
-                if (b < first || b >= first + out_width) out_table[(size_t)seq * table_width + b] = nowhere;
+                if (b < first || b >= first + out_width) out_table[(size_t)seq * table_width + b] = SEEN ? seq * out_width : 0;
     }
-    const int begin = max(0, oldest - logical * block_size), rows = min(block_size, ctx - logical * block_size);      // live rows of this block
-    const int block = logical < table_width && rows > begin ? block_table[(size_t)seq * table_width + logical] : 0;
+    const int begin = SEEN ? max(0, oldest - logical * block_size) : 0, rows = min(block_size, ctx - logical * block_size) - begin;     // live rows of this block (none: not positive)
+    const int block = logical < table_width && rows > 0 ? block_table[(size_t)seq * table_width + logical] : 0;
     const size_t from = ((size_t)block * num_kv_heads + kv_head) * block_size;
     const size_t to = ((size_t)blockIdx.x * num_kv_heads + kv_head) * block_size;
     const int words = head_dim >> 3, of_one = block_size * words;          // words of eight numbers
@@ -170,7 +173,7 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict
             const int idx = first_item + u * UNPACK_THREADS;
             const bool value = idx >= of_one;
             const int at = idx - (value ? of_one : 0), row = at / words, w = at - row * words;
-            const bool live = idx < 2 * of_one && row >= begin && row < rows;
+            const bool live = idx < 2 * of_one && (SEEN ? (uint32_t)(row - begin) < (uint32_t)max(0, rows) : row < rows);
             word[u] = live ? *(const uint32_t*)((value ? v_codes : k_codes) + (from + row) * (head_dim >> 1) + 4 * w) : 0u;
             byte[u] = live ? (value ? v_scale : k_scale)[(from + row) * (head_dim >> 4) + (w >> 1)] : 0u;
             target[u] = (to + row) * head_dim + 8 * w;
@@ -236,7 +239,7 @@ static int unpack_kv4(const char* name, const void* k_codes, const void* v_codes
     const long long items = 2ll * block_size * (head_dim / 8);
     if (items > 0x40000000ll) return fail(name, "a cache block is too large");
     const long long wanted = (items + UNPACK_ITEMS * UNPACK_THREADS - 1) / (UNPACK_ITEMS * UNPACK_THREADS), parts = wanted < 64 ? wanted : 64;
-    return launch_pdl(name, kv4_unpack_kernel, dim3((unsigned)(n_seqs * out_width), (unsigned)num_kv_heads, (unsigned)parts), dim3(UNPACK_THREADS), 0,
+    return launch_pdl(name, cu_q ? kv4_unpack_kernel<true> : kv4_unpack_kernel<false>, dim3((unsigned)(n_seqs * out_width), (unsigned)num_kv_heads, (unsigned)parts), dim3(UNPACK_THREADS), 0,
                       stream, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_table,
                       table_width, ctx_after, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, out_table, out_width, num_kv_heads, head_dim,
                       block_size, keep, cu_q, most_new, window, tile);
