@@ -1596,9 +1596,11 @@ class Kernels:
     def attention_kv4(self, q, k_codes, v_codes, k_scale, v_scale, block_table, cu_q, ctx_after, out, max_q_len: int, num_heads: int,
                       num_kv_heads: int, head_dim: int, block_size: int, scale: float, window: int = 0, scratch=None, flag=None):
         """Causal attention over a cache held in 4 bits (bfloat16 build): sequence ``s`` owns rows ``cu_q[s]..cu_q[s+1]-1`` of
-        ``q``/``out`` (at most ``max_q_len``), ``ctx_after[s]`` positions are cached, this step's included; ``scale`` is positive.  One or a few new tokens a sequence
-        read the cache as it lies; many read the bfloat16 numbers it stands for (``unpack_kv4``, then
-        ``attention_prefill_tc``, by which a value's NaN reaches all queries of a tile, as over a 16-bit cache).  ``scratch``: uint8, at least ``attention_kv4_scratch`` bytes; two steps that may run at once need one each.
+        ``q``/``out`` (at most ``max_q_len``), ``ctx_after[s]`` positions are cached, this step's included (a length beyond the table is cut to it);
+        ``scale`` is positive.  One or a few new tokens a sequence read the cache as it lies, with probabilities of 11 bits; many read the bfloat16
+        numbers it stands for, with probabilities of 8 bits (``attention_prefill_tc``, by which a value's NaN reaches all queries of a tile of its
+        sequence, as over a 16-bit cache).  Entries of blocks that no new token sees are not read.  ``scratch``: uint8, at least
+        ``attention_kv4_scratch`` bytes; two steps that may run at once need one each.
         A step's sums are cut by all its sequences' lengths, so that a sequence's result may differ in their order between batches."""
         u8, i32 = torch.uint8, torch.int32
         self._want_all("attention_kv4", (q, self.dtype, "q"), (out, self.dtype, "out"), (k_codes, u8, "k_codes"), (v_codes, u8, "v_codes"),
