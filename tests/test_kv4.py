@@ -261,3 +261,20 @@ def test_prompts_ask_for_scratch_within_its_bound():
                             position=SimpleNamespace(fusion_table=lambda n: None))
     PagedAttention._attend_in_4_bits(mixer, step, torch.zeros(300, 512), None, 0, True)
     assert asked["kv4_scratch"] == ((3000,), ops.KV4_UNPACKED)
+
+
+def test_reading_back_what_is_seen_refuses_bad_sizes():
+    lib = library("bfloat16", 64)
+    null, i = ctypes.c_void_p(0), ctypes.c_int
+
+    def seen(cu=ctypes.c_void_p(4), most=1, window=0, tile=64, seqs=1, width=1, dim=64, block=16, kv=2):
+        code = lib.skv_unpack_kv4_seen(null, null, null, null, null, i(1), null, null, null, null, i(seqs), i(width), i(kv), i(dim), i(block), cu, i(most),
+                                       i(window), i(tile), null)
+        return code, lib.skv_last_error().decode()
+
+    assert seen(seqs=0)[0] == 0 and seen(width=0, cu=null)[0] == 0
+    for match, changes in (("offsets", dict(cu=null)), ("must not be negative", dict(most=-1)), ("must not be negative", dict(window=-1)), ("positive tile", dict(tile=0)),
+                           ("multiple of 16", dict(dim=40)), ("block_size", dict(block=8)), ("kv heads", dict(kv=0)), ("too many", dict(seqs=2 ** 20, width=2 ** 12))):
+        code, message = seen(**changes)
+        assert code != 0 and match in message and "skv_unpack_kv4_seen" in message, (changes, message)
+    assert library("float32", 64).skv_unpack_kv4_seen(*([null] * 5), i(1), *([null] * 4), i(1), i(1), i(1), i(64), i(16), null, i(1), i(0), i(64), null) != 0
